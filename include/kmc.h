@@ -324,6 +324,75 @@ int kmc_colsums(const float *X, int64_t n, int d, const uint32_t *colmax, int64_
 int kmc_standardize(float *X, int64_t n, int d, const int64_t *sums, const uint32_t *colmax, int64_t n_total,
                     double *mean_std, void *stream);
 
+/* ---------------------------------------------------------------- routed experts
+ * No counterpart in the reference, whose answer is the one nearest center of a row: here a row (token) goes to its k
+ * best of E experts -- fitted centers, or any gate's scores -- and gets a weighted sum of their products.  The pieces
+ * are separate calls on plain arrays: kmc_route (choices and weights from logits), kmc_group_rows (the pairs
+ * (row, choice) grouped by expert), kmc_expert_matmul (each group times its expert's matrix), kmc_combine (the
+ * weighted sum per row), each with its gradient.  Sums are float32; 16-bit results are rounded once, when stored.
+ * Results do not depend on the order in which anything ran.  Rows, positions and pairs are counted in int32 (at most
+ * 2^31 - 1); byte offsets are 64-bit.  Dense arrays unless a row stride is given (in elements). */
+enum kmc_dtype { KMC_F32 = 0, KMC_BF16 = 1, KMC_F16 = 2 };
+
+#define KMC_MAX_ROUTE_EXPERTS 1024   /* experts of kmc_route */
+#define KMC_MAX_CHOICES 32           /* choices a row (kmc_route) */
+#define KMC_MAX_EXPERTS 4096         /* experts of kmc_group_rows and kmc_expert_matmul */
+
+#define KMC_ROUTE_SIGMOID 1u         /* scores sigma(logit) instead of a softmax */
+#define KMC_ROUTE_RENORM 2u          /* weights over the chosen experts only */
+
+/* ids (rows x choices int32) and weights (rows x choices float32) of logits (rows x experts of `dtype`, rows `stride`
+ * apart).  Expert i of a row is available when logit_i > -inf and key_i > -inf (so a NaN is not), key_i = logit_i
+ * (softmax) or 1 / (1 + exp(-logit_i)) (sigmoid), plus bias_i (experts float32, or NULL), in float32 with each
+ * operation rounded on its own, and when the row's mask byte (rows, or NULL) is not 0.  With groups > 1 (a divisor of
+ * experts, at most 32) only the top_groups groups of consecutive experts with the largest sum of their two best
+ * available keys stay.  ids are the largest keys in decreasing order, lowest index on ties, -1 (weight 0) where no
+ * available expert is left.  weights = scale * softmax of the logits (not the biased keys) over every expert whose
+ * logit is above -inf, or with KMC_ROUTE_RENORM over the chosen ones; scale * sigma(logit), with KMC_ROUTE_RENORM
+ * divided by the sum over the chosen (0 when that sum is 0).  A logit of +inf gives the softmax's NaN. */
+int kmc_route(const void *logits, int dtype, int64_t rows, int experts, int64_t stride, const float *bias,
+              const uint8_t *mask, int choices, int groups, int top_groups, float scale, unsigned flags, int32_t *ids,
+              float *weights, void *stream);
+/* dlogits (rows x experts of `dtype`, dense) from dweights (rows x choices float32): the derivative of kmc_route's
+ * weights for the ids it gave (distinct within a row; -1 has no part).  The choice itself has no derivative. */
+int kmc_route_grad(const float *dweights, const void *logits, int dtype, int64_t rows, int experts, int64_t stride,
+                   const int32_t *ids, int choices, float scale, unsigned flags, void *dlogits, void *stream);
+
+/* Stable grouping of pairs by expert.  ids: rows x choices int32 (labels of a Lloyd pass too: choices = 1); ids outside
+ * [0, experts) are left out.  offsets (experts + 1): expert e has positions offsets[e] .. offsets[e + 1] - 1, in
+ * increasing (row, choice).  group_row (rows * choices): the row of each position, -1 past offsets[experts].  slot
+ * (rows x choices): the position of each pair, or -1.  workspace: kmc_group_bytes(pairs, experts) bytes (may be 0). */
+size_t kmc_group_bytes(int64_t pairs, int experts);
+int kmc_group_rows(const int32_t *ids, int64_t rows, int choices, int experts, int32_t *offsets, int32_t *group_row,
+                   int32_t *slot, void *workspace, size_t ws_bytes, void *stream);
+
+/* y (pairs x n) = W_e x per position of expert e (offsets as kmc_group_rows gives them): x (x_rows x d, rows ldx apart),
+ * W (experts x n x d).  group_row: the row of x each position reads (a row outside x reads zeros); NULL: x is already
+ * grouped (x_rows = pairs).  Positions past offsets[experts] get zeros.  dtype KMC_BF16 or KMC_F16 throughout.
+ * kmc_expert_matmul_dx: dx (pairs x d) = W_e^T dy (pairs x n), by position (sum a row's positions with kmc_combine).
+ * kmc_expert_matmul_dw: dW (experts x n x d) = sum over an expert's positions of dy x^T; 0 for an expert with none.
+ * workspace: kmc_expert_bytes(...) bytes (may be 0), 256-byte aligned.  error (device int32, set to 0 once by the
+ * caller): 1 once a kernel gave up waiting on a barrier, its output then incomplete. */
+size_t kmc_expert_bytes(int64_t x_rows, int64_t pairs, int experts, int n, int d);
+int kmc_expert_matmul(const void *x, int64_t x_rows, int64_t ldx, const int32_t *group_row, const void *w,
+                      const int32_t *offsets, int64_t pairs, int experts, int n, int d, int dtype, void *y,
+                      void *workspace, size_t ws_bytes, int32_t *error, void *stream);
+int kmc_expert_matmul_dx(const void *dy, const void *w, const int32_t *offsets, int64_t pairs, int experts, int n,
+                         int d, int dtype, void *dx, void *workspace, size_t ws_bytes, int32_t *error, void *stream);
+int kmc_expert_matmul_dw(const void *dy, const void *x, int64_t x_rows, int64_t ldx, const int32_t *group_row,
+                         const int32_t *offsets, int64_t pairs, int experts, int n, int d, int dtype, void *dw,
+                         void *workspace, size_t ws_bytes, int32_t *error, void *stream);
+
+/* out (rows x width) = sum over a row's choices of weight * y[slot] (y: rows * choices x width of `dtype`, by
+ * position; weights: rows x choices float32, NULL: 1; a slot of -1 adds nothing).  kmc_combine_grad: dy (by position;
+ * zeros from position *taken on, taken = offsets + experts of the plan, device) = weight * dout, and dweights (rows x
+ * choices float32, NULL to skip) = <dout, y[slot]>, 0 for a slot of -1. */
+int kmc_combine(const void *y, int dtype, int64_t rows, int choices, int width, const int32_t *slot,
+                const float *weights, void *out, void *stream);
+int kmc_combine_grad(const void *dout, const void *y, int dtype, int64_t rows, int choices, int width,
+                     const int32_t *slot, const float *weights, const int32_t *taken, void *dy, float *dweights,
+                     void *stream);
+
 #ifdef __cplusplus
 }
 #endif

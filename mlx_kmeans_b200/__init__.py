@@ -13,7 +13,12 @@ from .core import (  # noqa: F401
     slice_rows, take_rows,
 )
 from .estimator import KMeans  # noqa: F401
+from .experts import (  # noqa: F401
+    RowGroups, combine_rows, combine_rows_grad, expert_matmul, expert_matmul_grad, expert_status, group_rows, route,
+    route_grad,
+)
 
 __version__ = "0.1.0"
 __all__ = ["KMeans", "Dataset", "kmeans", "lloyd_step", "assign_mlx", "assign", "kmeans_pp_init",
-           "make_data_numpy", "take_rows", "slice_rows"]
+           "make_data_numpy", "take_rows", "slice_rows", "RowGroups", "route", "route_grad", "group_rows",
+           "expert_matmul", "expert_matmul_grad", "expert_status", "combine_rows", "combine_rows_grad"]

@@ -18,6 +18,9 @@ KMC_PASS_LABEL32 = 4
 KMC_PASS_APPROX = 8
 KMC_PASS_ELKAN_BUILD = 16
 KMC_MAX_DIMS = 4096
+KMC_F32, KMC_BF16, KMC_F16 = 0, 1, 2
+KMC_ROUTE_SIGMOID = 1
+KMC_ROUTE_RENORM = 2
 STATS_BYTES = 64
 
 _vp = ctypes.c_void_p
@@ -26,6 +29,7 @@ _int = ctypes.c_int
 _u = ctypes.c_uint
 _u64 = ctypes.c_uint64
 _sz = ctypes.c_size_t
+_f = ctypes.c_float
 
 # name -> (restype, argtypes); mirrors include/kmc.h
 SIGNATURES = {
@@ -73,6 +77,18 @@ SIGNATURES = {
                        ctypes.c_float, _vp]),
     "kmc_colsums": (_int, [_vp, _i64, _int, _vp, _i64, _vp, _vp]),
     "kmc_standardize": (_int, [_vp, _i64, _int, _vp, _vp, _i64, _vp, _vp]),
+    "kmc_route": (_int, [_vp, _int, _i64, _int, _i64, _vp, _vp, _int, _int, _int, _f, _u, _vp, _vp, _vp]),
+    "kmc_route_grad": (_int, [_vp, _vp, _int, _i64, _int, _i64, _vp, _int, _f, _u, _vp, _vp]),
+    "kmc_group_bytes": (_sz, [_i64, _int]),
+    "kmc_group_rows": (_int, [_vp, _i64, _int, _int, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "kmc_expert_bytes": (_sz, [_i64, _i64, _int, _int, _int]),
+    "kmc_expert_matmul": (_int, [_vp, _i64, _i64, _vp, _vp, _vp, _i64, _int, _int, _int, _int, _vp, _vp, _sz, _vp,
+                                 _vp]),
+    "kmc_expert_matmul_dx": (_int, [_vp, _vp, _vp, _i64, _int, _int, _int, _int, _vp, _vp, _sz, _vp, _vp]),
+    "kmc_expert_matmul_dw": (_int, [_vp, _vp, _i64, _i64, _vp, _vp, _i64, _int, _int, _int, _int, _vp, _vp, _sz, _vp,
+                                    _vp]),
+    "kmc_combine": (_int, [_vp, _int, _i64, _int, _int, _vp, _vp, _vp, _vp]),
+    "kmc_combine_grad": (_int, [_vp, _vp, _int, _i64, _int, _int, _vp, _vp, _vp, _vp, _vp, _vp]),
 }
 
 _lib = None

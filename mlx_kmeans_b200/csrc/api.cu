@@ -2,6 +2,7 @@
 // dispatch to the kernels, and the error reporting: every entry point returns a status and records a
 // message for kmc_last_error(); nothing is thrown across the ABI.
 #include <cstdarg>
+#include <cstdint>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
@@ -770,6 +771,277 @@ int kmc_pass_static(const float* X, int64_t n, int d, const float* C, int k, con
     if (int s = static_scratch("kmc_pass_static", &ws)) return s;
     return kmc_pass(X, n, d, C, k, colmax, n_total, totals, labels, best, flags, ws, (size_t)KMC_STATIC_SCRATCH_BYTES,
                     stream);
+}
+
+// ---------------------------------------------------------------- routed experts
+
+static int check_dtype(const char* who, int dtype, bool f32) {
+    if (dtype == KMC_BF16 || dtype == KMC_F16 || (f32 && dtype == KMC_F32)) return KMC_OK;
+    return fail(KMC_ERR_INVALID, "%s: dtype %d is not %s", who, dtype, f32 ? "float32, bfloat16 or float16" : "bfloat16 or float16");
+}
+
+// rows of `choices` pairs, counted in int32
+static int check_pairs(const char* who, int64_t rows, int choices) {
+    if (rows < 0) return fail(KMC_ERR_INVALID, "%s: rows must be >= 0, got %lld", who, (long long)rows);
+    if (choices < 1) return fail(KMC_ERR_INVALID, "%s: choices must be >= 1, got %d", who, choices);
+    if (rows > INT32_MAX / choices)
+        return fail(KMC_ERR_UNSUPPORTED, "%s: %lld rows of %d choices are more than 2^31 - 1 pairs", who, (long long)rows, choices);
+    return KMC_OK;
+}
+
+static int check_route(const char* who, int dtype, int64_t rows, int experts, int64_t stride, int choices, unsigned flags) {
+    if (int s = check_dtype(who, dtype, true)) return s;
+    if (int s = check_pairs(who, rows, choices)) return s;
+    if (experts < 1) return fail(KMC_ERR_INVALID, "%s: experts must be >= 1, got %d", who, experts);
+    if (experts > KMC_MAX_ROUTE_EXPERTS)
+        return fail(KMC_ERR_UNSUPPORTED, "%s: %d experts, above the supported maximum %d", who, experts, KMC_MAX_ROUTE_EXPERTS);
+    if (choices > experts) return fail(KMC_ERR_INVALID, "%s: %d choices of %d experts", who, choices, experts);
+    if (choices > KMC_MAX_CHOICES)
+        return fail(KMC_ERR_UNSUPPORTED, "%s: %d choices, above the supported maximum %d", who, choices, KMC_MAX_CHOICES);
+    if (stride < experts) return fail(KMC_ERR_INVALID, "%s: rows %lld apart hold %d experts", who, (long long)stride, experts);
+    if (flags & ~(KMC_ROUTE_SIGMOID | KMC_ROUTE_RENORM)) return fail(KMC_ERR_INVALID, "%s: unknown flags %u", who, flags);
+    return KMC_OK;
+}
+
+int kmc_route(const void* logits, int dtype, int64_t rows, int experts, int64_t stride, const float* bias,
+              const uint8_t* mask, int choices, int groups, int top_groups, float scale, unsigned flags, int32_t* ids,
+              float* weights, void* stream) {
+    if (int s = check_route("kmc_route", dtype, rows, experts, stride, choices, flags)) return s;
+    if (groups < 1 || groups > 32 || experts % groups != 0)
+        return fail(KMC_ERR_INVALID, "kmc_route: %d groups of %d experts (a divisor, at most 32, is wanted)", groups, experts);
+    if (top_groups < 1 || top_groups > groups)
+        return fail(KMC_ERR_INVALID, "kmc_route: the best %d of %d groups", top_groups, groups);
+    if (rows > 0 && (!logits || !ids || !weights)) return fail(KMC_ERR_INVALID, "kmc_route: null pointer");
+    if (rows == 0) return KMC_OK;
+    RouteCall c = {};
+    c.logits = logits;
+    c.dtype = dtype;
+    c.rows = rows;
+    c.stride = stride;
+    c.experts = experts;
+    c.choices = choices;
+    c.groups = groups;
+    c.top_groups = top_groups;
+    c.bias = bias;
+    c.mask = mask;
+    c.scale = scale;
+    c.sigmoid = (flags & KMC_ROUTE_SIGMOID) != 0;
+    c.renorm = (flags & KMC_ROUTE_RENORM) != 0;
+    c.ids_out = ids;
+    c.weights = weights;
+    cudaError_t e = launch_route(c, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "kmc_route");
+    return KMC_OK;
+}
+
+int kmc_route_grad(const float* dweights, const void* logits, int dtype, int64_t rows, int experts, int64_t stride,
+                   const int32_t* ids, int choices, float scale, unsigned flags, void* dlogits, void* stream) {
+    if (int s = check_route("kmc_route_grad", dtype, rows, experts, stride, choices, flags)) return s;
+    if (rows > 0 && (!dweights || !logits || !ids || !dlogits)) return fail(KMC_ERR_INVALID, "kmc_route_grad: null pointer");
+    if (rows == 0) return KMC_OK;
+    RouteCall c = {};
+    c.logits = logits;
+    c.dtype = dtype;
+    c.rows = rows;
+    c.stride = stride;
+    c.experts = experts;
+    c.choices = choices;
+    c.groups = 1;
+    c.top_groups = 1;
+    c.scale = scale;
+    c.sigmoid = (flags & KMC_ROUTE_SIGMOID) != 0;
+    c.renorm = (flags & KMC_ROUTE_RENORM) != 0;
+    c.dweights = dweights;
+    c.ids = ids;
+    c.dlogits = dlogits;
+    cudaError_t e = launch_route(c, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "kmc_route_grad");
+    return KMC_OK;
+}
+
+static int check_experts(const char* who, int experts) {
+    if (experts < 1) return fail(KMC_ERR_INVALID, "%s: experts must be >= 1, got %d", who, experts);
+    if (experts > KMC_MAX_EXPERTS)
+        return fail(KMC_ERR_UNSUPPORTED, "%s: %d experts, above the supported maximum %d", who, experts, KMC_MAX_EXPERTS);
+    return KMC_OK;
+}
+
+size_t kmc_group_bytes(int64_t pairs, int experts) { return pairs > 0 && experts > 0 ? group_bytes(pairs, experts) : 0; }
+
+int kmc_group_rows(const int32_t* ids, int64_t rows, int choices, int experts, int32_t* offsets, int32_t* group_row,
+                   int32_t* slot, void* workspace, size_t ws_bytes, void* stream) {
+    if (int s = check_pairs("kmc_group_rows", rows, choices)) return s;
+    if (int s = check_experts("kmc_group_rows", experts)) return s;
+    if (!offsets || (rows > 0 && (!ids || !group_row || !slot))) return fail(KMC_ERR_INVALID, "kmc_group_rows: null pointer");
+    const size_t need = group_bytes(rows * choices, experts);
+    if (need > 0 && (!workspace || ws_bytes < need))
+        return fail(KMC_ERR_INVALID, "kmc_group_rows: workspace of %zu bytes, need %zu", workspace ? ws_bytes : (size_t)0, need);
+    cudaError_t e = launch_group(ids, rows * choices, choices, experts, offsets, group_row, slot, workspace,
+                                 static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "kmc_group_rows");
+    return KMC_OK;
+}
+
+static int check_expert(const char* who, int64_t pairs, int experts, int n, int d, int dtype, const void* offsets,
+                        const void* error) {
+    if (int s = check_dtype(who, dtype, false)) return s;
+    if (int s = check_pairs(who, pairs, 1)) return s;
+    if (int s = check_experts(who, experts)) return s;
+    if (n < 1 || d < 1) return fail(KMC_ERR_INVALID, "%s: matrices of %d x %d", who, n, d);
+    if (n > (1 << 20) || d > (1 << 20)) return fail(KMC_ERR_UNSUPPORTED, "%s: matrices of %d x %d, above 2^20", who, n, d);
+    if (!offsets || !error) return fail(KMC_ERR_INVALID, "%s: null pointer", who);
+    return KMC_OK;
+}
+
+static int run_expert(const char* who, const ExpertCall& c, size_t ws_bytes, void* stream) {
+    const size_t need = expert_bytes(c);
+    if (need > 0 && (!c.ws || ws_bytes < need))
+        return fail(KMC_ERR_INVALID, "%s: workspace of %zu bytes, need %zu", who, c.ws ? ws_bytes : (size_t)0, need);
+    cudaError_t e = launch_expert(c, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, who);
+    return KMC_OK;
+}
+
+int kmc_expert_matmul(const void* x, int64_t x_rows, int64_t ldx, const int32_t* group_row, const void* w,
+                      const int32_t* offsets, int64_t pairs, int experts, int n, int d, int dtype, void* y,
+                      void* workspace, size_t ws_bytes, int32_t* error, void* stream) {
+    if (int s = check_expert("kmc_expert_matmul", pairs, experts, n, d, dtype, offsets, error)) return s;
+    if (int s = check_pairs("kmc_expert_matmul", x_rows, 1)) return s;
+    if (ldx < d) return fail(KMC_ERR_INVALID, "kmc_expert_matmul: rows %lld apart hold %d columns", (long long)ldx, d);
+    if (!group_row && x_rows != pairs)
+        return fail(KMC_ERR_INVALID, "kmc_expert_matmul: %lld grouped rows for %lld positions", (long long)x_rows, (long long)pairs);
+    if (!w || (pairs > 0 && !y) || (x_rows > 0 && !x)) return fail(KMC_ERR_INVALID, "kmc_expert_matmul: null pointer");
+    if (pairs == 0) return KMC_OK;
+    ExpertCall c = {};
+    c.kind = kExpertForward;
+    c.dtype = dtype;
+    c.x = x;
+    c.x_rows = x_rows;
+    c.ldx = ldx;
+    c.rows = group_row;
+    c.w = w;
+    c.offsets = offsets;
+    c.pairs = pairs;
+    c.experts = experts;
+    c.n = n;
+    c.d = d;
+    c.y = y;
+    c.ws = workspace;
+    c.error = error;
+    return run_expert("kmc_expert_matmul", c, ws_bytes, stream);
+}
+
+int kmc_expert_matmul_dx(const void* dy, const void* w, const int32_t* offsets, int64_t pairs, int experts, int n,
+                         int d, int dtype, void* dx, void* workspace, size_t ws_bytes, int32_t* error, void* stream) {
+    if (int s = check_expert("kmc_expert_matmul_dx", pairs, experts, n, d, dtype, offsets, error)) return s;
+    if (!w || (pairs > 0 && (!dy || !dx))) return fail(KMC_ERR_INVALID, "kmc_expert_matmul_dx: null pointer");
+    if (pairs == 0) return KMC_OK;
+    ExpertCall c = {};
+    c.kind = kExpertDx;
+    c.dtype = dtype;
+    c.dy = dy;
+    c.w = w;
+    c.offsets = offsets;
+    c.pairs = pairs;
+    c.experts = experts;
+    c.n = n;
+    c.d = d;
+    c.dx = dx;
+    c.ws = workspace;
+    c.error = error;
+    return run_expert("kmc_expert_matmul_dx", c, ws_bytes, stream);
+}
+
+int kmc_expert_matmul_dw(const void* dy, const void* x, int64_t x_rows, int64_t ldx, const int32_t* group_row,
+                         const int32_t* offsets, int64_t pairs, int experts, int n, int d, int dtype, void* dw,
+                         void* workspace, size_t ws_bytes, int32_t* error, void* stream) {
+    if (int s = check_expert("kmc_expert_matmul_dw", pairs, experts, n, d, dtype, offsets, error)) return s;
+    if (int s = check_pairs("kmc_expert_matmul_dw", x_rows, 1)) return s;
+    if (ldx < d) return fail(KMC_ERR_INVALID, "kmc_expert_matmul_dw: rows %lld apart hold %d columns", (long long)ldx, d);
+    if (!group_row && x_rows != pairs)
+        return fail(KMC_ERR_INVALID, "kmc_expert_matmul_dw: %lld grouped rows for %lld positions", (long long)x_rows, (long long)pairs);
+    if (!dw || (pairs > 0 && !dy) || (x_rows > 0 && !x)) return fail(KMC_ERR_INVALID, "kmc_expert_matmul_dw: null pointer");
+    ExpertCall c = {};
+    c.kind = kExpertDw;
+    c.dtype = dtype;
+    c.dy = dy;
+    c.x = x;
+    c.x_rows = x_rows;
+    c.ldx = ldx;
+    c.rows = group_row;
+    c.offsets = offsets;
+    c.pairs = pairs;
+    c.experts = experts;
+    c.n = n;
+    c.d = d;
+    c.dw = dw;
+    c.ws = workspace;
+    c.error = error;
+    return run_expert("kmc_expert_matmul_dw", c, ws_bytes, stream);
+}
+
+size_t kmc_expert_bytes(int64_t x_rows, int64_t pairs, int experts, int n, int d) {
+    ExpertCall c = {};
+    c.x_rows = x_rows > 0 ? x_rows : 0;
+    c.pairs = pairs > 0 ? pairs : 0;
+    c.experts = experts > 0 ? experts : 0;
+    c.n = n > 0 ? n : 0;
+    c.d = d > 0 ? d : 0;
+    return expert_bytes(c);
+}
+
+static int check_combine(const char* who, int dtype, int64_t rows, int choices, int width) {
+    if (int s = check_dtype(who, dtype, true)) return s;
+    if (int s = check_pairs(who, rows, choices)) return s;
+    if (width < 1) return fail(KMC_ERR_INVALID, "%s: width must be >= 1, got %d", who, width);
+    if (width > (1 << 20)) return fail(KMC_ERR_UNSUPPORTED, "%s: width %d, above 2^20", who, width);
+    // one block per 256 elements at the least favourable alignment: the grid's limit of 2^31 - 1 blocks
+    if (rows * (int64_t)width / 256 >= INT32_MAX)
+        return fail(KMC_ERR_UNSUPPORTED, "%s: %lld rows of %d features", who, (long long)rows, width);
+    return KMC_OK;
+}
+
+int kmc_combine(const void* y, int dtype, int64_t rows, int choices, int width, const int32_t* slot,
+                const float* weights, void* out, void* stream) {
+    if (int s = check_combine("kmc_combine", dtype, rows, choices, width)) return s;
+    if (rows > 0 && (!y || !slot || !out)) return fail(KMC_ERR_INVALID, "kmc_combine: null pointer");
+    if (rows == 0) return KMC_OK;
+    CombineCall c = {};
+    c.y = y;
+    c.slot = slot;
+    c.weights = weights;
+    c.tokens = rows;
+    c.choices = choices;
+    c.width = width;
+    c.dtype = dtype;
+    c.out = out;
+    cudaError_t e = launch_combine(c, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "kmc_combine");
+    return KMC_OK;
+}
+
+int kmc_combine_grad(const void* dout, const void* y, int dtype, int64_t rows, int choices, int width,
+                     const int32_t* slot, const float* weights, const int32_t* taken, void* dy, float* dweights,
+                     void* stream) {
+    if (int s = check_combine("kmc_combine_grad", dtype, rows, choices, width)) return s;
+    if (rows > 0 && (!dout || !slot || !taken || !dy || (dweights && !y)))
+        return fail(KMC_ERR_INVALID, "kmc_combine_grad: null pointer");
+    if (rows == 0) return KMC_OK;
+    CombineCall c = {};
+    c.y = y;
+    c.slot = slot;
+    c.weights = weights;
+    c.tokens = rows;
+    c.choices = choices;
+    c.width = width;
+    c.dtype = dtype;
+    c.dout = dout;
+    c.taken = taken;
+    c.dy = dy;
+    c.dweights = dweights;
+    cudaError_t e = launch_combine(c, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "kmc_combine_grad");
+    return KMC_OK;
 }
 
 }  // extern "C"

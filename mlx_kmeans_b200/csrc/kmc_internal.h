@@ -213,4 +213,61 @@ cudaError_t launch_colsums(const float* X, int64_t n, int d, const unsigned int*
 cudaError_t launch_standardize(float* X, int64_t n, int d, const long long* sums, const unsigned int* colmax,
                                int64_t n_total, double* mean_std, cudaStream_t st);
 
+// Routed experts: routing (route.cu), the grouping plan (group.cu), products per expert (expert_*.cu), combination
+// (combine.cu).  dtype: the public kmc_dtype.
+struct RouteCall {
+    const void* logits;
+    int dtype;
+    int64_t rows, stride;
+    int experts, choices, groups, top_groups;
+    const float* bias;
+    const uint8_t* mask;
+    float scale;
+    int sigmoid, renorm;
+    int32_t* ids_out;         // forward
+    float* weights;
+    const float* dweights;    // gradient (nullptr: forward)
+    const int32_t* ids;
+    void* dlogits;
+};
+cudaError_t launch_route(const RouteCall& c, cudaStream_t st);
+
+constexpr int kGroupMaxExperts = 4096;
+size_t group_bytes(int64_t pairs, int experts);
+cudaError_t launch_group(const int32_t* ids, int64_t pairs, int choices, int experts, int32_t* offsets, int32_t* rows,
+                         int32_t* slot, void* ws, cudaStream_t st);
+
+struct CombineCall {
+    const void* y;            // pairs x width
+    const int32_t* slot;      // tokens x choices
+    const float* weights;     // tokens x choices, or nullptr: 1
+    int64_t tokens;
+    int choices, width, dtype;
+    void* out;                // forward: tokens x width
+    const void* dout;         // gradient (nullptr: forward)
+    const int32_t* taken;     // device: positions with a pair
+    void* dy;
+    float* dweights;          // or nullptr
+};
+cudaError_t launch_combine(const CombineCall& c, cudaStream_t st);
+
+enum ExpertKind { kExpertForward, kExpertDx, kExpertDw };
+struct ExpertCall {
+    ExpertKind kind;
+    int dtype;                // bfloat16 or float16
+    const void* x;            // x_rows x d, rows ldx apart
+    int64_t x_rows, ldx;
+    const int32_t* rows;      // row of x per position, or nullptr: the position itself
+    const void* w;            // experts x n x d
+    const void* dy;           // pairs x n
+    const int32_t* offsets;   // experts + 1
+    int64_t pairs;
+    int experts, n, d;
+    void *y, *dx, *dw;        // the output of each kind
+    void* ws;                 // expert_bytes(call) bytes
+    int* error;               // set to 1 by a kernel that gave up on a barrier
+};
+size_t expert_bytes(const ExpertCall& c);
+cudaError_t launch_expert(const ExpertCall& c, cudaStream_t st);
+
 }  // namespace kmc

@@ -1,0 +1,356 @@
+// route.cu -- routing of rows to their top-k experts (kmc_route) and the gradient of the weights (kmc_route_grad).
+//
+// The top-1 label of a Lloyd pass generalised to the k best of E scores with weights.  Row t, logits l_0 .. l_{E-1}:
+//   key_i  = l_i (softmax) or sigma(l_i) = 1 / (1 + exp(-l_i)) (sigmoid), plus bias_i; float32, each operation
+//            rounded on its own, so the choice is defined bit for bit.  Expert i is available when l_i > -inf and
+//            key_i > -inf (a NaN is not) and the row's mask is set.
+//   groups   with G > 1 groups of E / G consecutive experts, a group scores the sum of its two best available keys
+//            (its best, when it has one); only the top_groups best groups stay (lowest index on ties).
+//   ids      the k largest keys in decreasing order, lowest index on ties; -1 where no available expert is left.
+//   weights  softmax over the available logits, or (RENORM) over the chosen ones; sigma(l_id), or (RENORM) divided by
+//            the sum over the chosen (0 when that sum is 0); times `scale`.
+// Gradient, with g = scale dL/dweights on the chosen (the choice itself, and so the bias, has none):
+//   softmax  dl_i = p_i ([i chosen] g_i - sum_j g_j p_j) over the available, RENORM: over the chosen, 0 elsewhere
+//   sigmoid  dl_i = g_i s_i (1 - s_i), RENORM: (g_i - sum_j g_j s_j / S) / S  s_i (1 - s_i), S = sum of the chosen s_j
+//
+// One warp owns a row: lane L holds the PER consecutive experts from L PER on (PER = 1, 2, 4 .. 32: E up to 1024),
+// read with 16-byte loads where the row allows, as order-preserving 32-bit integers (0: not available).  A choice is
+// one redux.max over the lanes' best, a ballot whose first lane has the lowest index, and a rescan by that lane.
+// Memory or launch bound: E reads and 8 k bytes written per row.
+#include "common.cuh"
+#include "experts.cuh"
+#include "kmc_internal.h"
+
+namespace kmc {
+
+namespace {
+
+constexpr unsigned kFull = 0xffffffffu;
+constexpr int kRouteWarps = 8;
+
+// float order as unsigned order (-0 first made +0; no NaN comes here); every finite or infinite value maps above 0
+__device__ __forceinline__ unsigned ordered(float f) {
+    const unsigned u = __float_as_uint(__fadd_rn(f, 0.0f));
+    return u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float unordered(unsigned u) {
+    return __uint_as_float((u & 0x80000000u) ? (u ^ 0x80000000u) : ~u);
+}
+__device__ __forceinline__ float sigmoid32(float l) { return __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-l))); }
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+    return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
+    return v;
+}
+
+// The lane's PER logits of one row (-inf past the last expert).  vec: the row starts on a 16-byte boundary, or on
+// one of PER elements where that is less.
+template <typename T, int PER>
+__device__ __forceinline__ void load_row(const T* row, int experts, bool vec, float (&l)[PER]) {
+    constexpr int V = PER * sizeof(T) >= 16 ? 16 / sizeof(T) : PER;
+    const int i0 = (threadIdx.x & 31) * PER;
+#pragma unroll
+    for (int i = 0; i < PER; i += V) {
+        if (vec && i0 + i + V <= experts) {
+            const Pack<T, V> p = *reinterpret_cast<const Pack<T, V>*>(row + i0 + i);
+#pragma unroll
+            for (int j = 0; j < V; j++) l[i + j] = Elem<T>::to(p.v[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; j++) l[i + j] = i0 + i + j < experts ? Elem<T>::to(row[i0 + i + j]) : -INFINITY;
+        }
+    }
+}
+
+struct RouteArgs {
+    int64_t rows, stride;
+    int experts, choices, groups, top_groups, group_size;
+    const float* bias;
+    const uint8_t* mask;
+    float scale;
+    int sigmoid, renorm;
+    int vec, out_vec;                                      // rows of logits / dlogits allow whole-vector accesses
+};
+
+// Clears the keys of experts outside the best top_groups groups.  A group that covers a power of two of whole lanes
+// merges its lanes' two best keys by xor shuffles; any other split of the experts goes group by group with a masked
+// rescan (8 groups of 256 experts: 45 instructions a row against about 500).
+template <int PER>
+__device__ __forceinline__ void keep_groups(const RouteArgs& a, unsigned (&key)[PER]) {
+    const int lane = threadIdx.x & 31, gs = a.group_size, G = a.groups;
+    unsigned mine = 0u;                                    // lane g: group g's best key, then its score
+    unsigned second = 0u;
+    const int lanes = gs / PER;
+    if (gs % PER == 0 && (lanes & (lanes - 1)) == 0) {
+        unsigned b0 = 0u, b1 = 0u;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            b1 = max(b1, min(b0, key[i]));
+            b0 = max(b0, key[i]);
+        }
+        for (int o = 1; o < lanes; o <<= 1) {
+            const unsigned c0 = __shfl_xor_sync(kFull, b0, o), c1 = __shfl_xor_sync(kFull, b1, o);
+            b1 = max(max(b1, c1), min(b0, c0));
+            b0 = max(b0, c0);
+        }
+        const int src = lane < G ? lane * lanes : 0;       // G lanes <= 32 PER / PER: in range
+        mine = __shfl_sync(kFull, b0, src);
+        second = __shfl_sync(kFull, b1, src);
+    } else {
+        for (int g = 0; g < G; g++) {
+            unsigned b0 = 0u, b1 = 0u;
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const int e = lane * PER + i - g * gs;
+                const unsigned v = e >= 0 && e < gs ? key[i] : 0u;
+                b1 = max(b1, min(b0, v));
+                b0 = max(b0, v);
+            }
+            const unsigned m0 = __reduce_max_sync(kFull, b0);
+            const int first = __ffs(__ballot_sync(kFull, b0 == m0)) - 1;
+            const unsigned m1 = __reduce_max_sync(kFull, lane == first ? b1 : b0);
+            if (lane == g) {
+                mine = m0;
+                second = m1;
+            }
+        }
+    }
+    const bool some = lane < G && mine != 0u;
+    const float best = some ? unordered(mine) : -INFINITY;
+    const float score = some && second != 0u ? __fadd_rn(best, unordered(second)) : best;
+    int rank = 0;
+    for (int g = 0; g < G; g++) {
+        const float s = __shfl_sync(kFull, score, g);
+        rank += (s > score || (s == score && g < lane)) ? 1 : 0;
+    }
+    const unsigned keep = __ballot_sync(kFull, some && rank < a.top_groups);
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int g = (lane * PER + i) / gs;
+        if (g >= G || !((keep >> g) & 1u)) key[i] = 0u;
+    }
+}
+
+template <typename T, int PER>
+__global__ void __launch_bounds__(kRouteWarps * 32)
+    k_route(const T* __restrict__ logits, RouteArgs a, int32_t* __restrict__ ids, float* __restrict__ weights) {
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int64_t t = (int64_t)blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
+    if (t >= a.rows) return;
+    const T* row = logits + t * a.stride;
+    float l[PER];
+    load_row<T, PER>(row, a.experts, a.vec, l);
+    const bool live = a.mask == nullptr || a.mask[t] != 0;
+    unsigned key[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int e = lane * PER + i;
+        float v = a.sigmoid ? sigmoid32(l[i]) : l[i];
+        if (a.bias != nullptr && e < a.experts) v = __fadd_rn(v, a.bias[e]);
+        key[i] = live && l[i] > -INFINITY && v > -INFINITY ? ordered(v) : 0u;
+    }
+    float m = 0.0f, total = 1.0f;
+    if (!a.sigmoid && !a.renorm) {                         // the softmax runs over every available logit
+        m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < PER; i++) m = l[i] > m ? l[i] : m;
+        m = warp_max(m);
+        total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PER; i++) total += l[i] > -INFINITY ? expf(l[i] - m) : 0.0f;
+        total = warp_sum(total);
+    }
+    if (a.groups > 1) keep_groups<PER>(a, key);
+
+    unsigned best = 0u;
+    int at = 0;
+#pragma unroll
+    for (int i = PER - 1; i >= 0; i--)
+        if (key[i] >= best) {                              // the lowest of equal keys
+            best = key[i];
+            at = i;
+        }
+    int mine = -1;                                         // lane j: the j-th choice
+    for (int j = 0; j < a.choices; j++) {
+        const unsigned top = __reduce_max_sync(kFull, best);
+        if (top == 0u) break;                              // nothing available is left
+        const int owner = __ffs(__ballot_sync(kFull, best == top)) - 1;
+        const int e = __shfl_sync(kFull, lane * PER + at, owner);
+        if (lane == j) mine = e;
+        if (lane == owner) {
+            best = 0u;
+            const int gone = at;
+#pragma unroll
+            for (int i = PER - 1; i >= 0; i--) {
+                if (i == gone) key[i] = 0u;
+                if (key[i] >= best) {
+                    best = key[i];
+                    at = i;
+                }
+            }
+        }
+    }
+    float w = 0.0f;
+    const bool got = mine >= 0;
+    const float lm = got ? Elem<T>::to(row[mine]) : -INFINITY;
+    if (a.sigmoid) {
+        const float s = got ? sigmoid32(lm) : 0.0f;
+        if (a.renorm) {
+            const float sum = warp_sum(s);
+            w = sum > 0.0f ? s / sum : 0.0f;
+        } else {
+            w = s;
+        }
+    } else {
+        if (a.renorm) m = warp_max(lm);
+        const float p = got ? expf(lm - m) : 0.0f;
+        if (a.renorm) total = warp_sum(p);
+        w = got ? p / total : 0.0f;
+    }
+    if (lane < a.choices) {
+        ids[t * a.choices + lane] = mine;
+        weights[t * a.choices + lane] = a.scale * w;
+    }
+}
+
+template <typename T, int PER>
+__global__ void __launch_bounds__(kRouteWarps * 32)
+    k_route_grad(const float* __restrict__ dweights, const T* __restrict__ logits, const int32_t* __restrict__ ids,
+                 RouteArgs a, T* __restrict__ dlogits) {
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int64_t t = (int64_t)blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
+    if (t >= a.rows) return;
+    const T* row = logits + t * a.stride;
+    T* out = dlogits + t * a.experts;
+    int id = lane < a.choices ? ids[t * a.choices + lane] : -1;
+    const bool got = id >= 0 && id < a.experts;
+    const float g = got ? a.scale * dweights[t * a.choices + lane] : 0.0f;
+    const float lm = got ? Elem<T>::to(row[id]) : -INFINITY;
+
+    float p, dot, m = 0.0f, total = 1.0f, slope = 0.0f;
+    if (a.sigmoid) {
+        const float s = got ? sigmoid32(lm) : 0.0f;
+        // 1 - s from exp(l): no cancellation where s is near 1
+        slope = got ? s * sigmoid32(-lm) : 0.0f;
+        p = s;
+        dot = 0.0f;
+        if (a.renorm) {
+            total = warp_sum(s);
+            dot = total > 0.0f ? warp_sum(g * s) / total : 0.0f;
+        }
+    } else if (a.renorm) {
+        m = warp_max(lm);
+        p = got ? expf(lm - m) : 0.0f;
+        total = warp_sum(p);
+        p = got ? p / total : 0.0f;
+        dot = warp_sum(g * p);
+    }
+    float dl[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++) dl[i] = 0.0f;
+    if (!a.sigmoid && !a.renorm) {
+        load_row<T, PER>(row, a.experts, a.vec, dl);
+        m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < PER; i++) m = dl[i] > m ? dl[i] : m;
+        m = warp_max(m);
+        total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            dl[i] = dl[i] > -INFINITY ? expf(dl[i] - m) : 0.0f;
+            total += dl[i];
+        }
+        total = warp_sum(total);
+        p = got ? expf(lm - m) / total : 0.0f;
+        dot = warp_sum(g * p);
+        const float c = __any_sync(kFull, got) ? -dot / total : 0.0f;   // a row with no choice: 0, whatever its logits
+#pragma unroll
+        for (int i = 0; i < PER; i++) dl[i] = dl[i] != 0.0f ? c * dl[i] : 0.0f;
+    }
+    // the dense row first, then the chosen entries over it
+    constexpr int V = PER * sizeof(T) >= 16 ? 16 / sizeof(T) : PER;
+    const int i0 = lane * PER;
+#pragma unroll
+    for (int i = 0; i < PER; i += V) {
+        if (a.out_vec && i0 + i + V <= a.experts) {
+            Pack<T, V> q;
+#pragma unroll
+            for (int j = 0; j < V; j++) q.v[j] = Elem<T>::from(dl[i + j]);
+            *reinterpret_cast<Pack<T, V>*>(out + i0 + i) = q;
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; j++)
+                if (i0 + i + j < a.experts) out[i0 + i + j] = Elem<T>::from(dl[i + j]);
+        }
+    }
+    __syncwarp();
+    if (got) {
+        float v;
+        if (a.sigmoid) {
+            v = !a.renorm ? g * slope : total > 0.0f ? (g - dot) / total * slope : 0.0f;
+        } else {
+            v = p * (g - dot);
+        }
+        out[id] = Elem<T>::from(v);
+    }
+}
+
+template <typename T, int PER>
+cudaError_t run_route(const RouteCall& c, const RouteArgs& a, cudaStream_t st) {
+    const int64_t blocks = (a.rows + kRouteWarps - 1) / kRouteWarps;
+    if (c.dweights == nullptr)
+        return launch_pdl(k_route<T, PER>, dim3((unsigned)blocks), dim3(kRouteWarps * 32), 0, st,
+                          static_cast<const T*>(c.logits), a, c.ids_out, c.weights);
+    return launch_pdl(k_route_grad<T, PER>, dim3((unsigned)blocks), dim3(kRouteWarps * 32), 0, st, c.dweights,
+                      static_cast<const T*>(c.logits), c.ids, a, static_cast<T*>(c.dlogits));
+}
+
+template <typename T>
+cudaError_t run_route_type(const RouteCall& c, cudaStream_t st) {
+    int per = 1;
+    while (per * 32 < c.experts) per *= 2;
+    RouteArgs a;
+    a.rows = c.rows;
+    a.stride = c.stride;
+    a.experts = c.experts;
+    a.choices = c.choices;
+    a.groups = c.groups;
+    a.top_groups = c.top_groups;
+    a.group_size = c.experts / (c.groups > 0 ? c.groups : 1);
+    a.bias = c.bias;
+    a.mask = c.mask;
+    a.scale = c.scale;
+    a.sigmoid = c.sigmoid;
+    a.renorm = c.renorm;
+    const size_t step = per * sizeof(T) >= 16 ? 16 : per * sizeof(T);
+    a.vec = reinterpret_cast<uintptr_t>(c.logits) % step == 0 && (c.stride * sizeof(T)) % step == 0;
+    a.out_vec = reinterpret_cast<uintptr_t>(c.dlogits) % step == 0 && (c.experts * sizeof(T)) % step == 0;
+    switch (per) {
+        case 1: return run_route<T, 1>(c, a, st);
+        case 2: return run_route<T, 2>(c, a, st);
+        case 4: return run_route<T, 4>(c, a, st);
+        case 8: return run_route<T, 8>(c, a, st);
+        case 16: return run_route<T, 16>(c, a, st);
+        default: return run_route<T, 32>(c, a, st);
+    }
+}
+
+}  // namespace
+
+cudaError_t launch_route(const RouteCall& c, cudaStream_t st) {
+    switch (c.dtype) {
+        case 0: return run_route_type<float>(c, st);
+        case 1: return run_route_type<__nv_bfloat16>(c, st);
+        default: return run_route_type<__half>(c, st);
+    }
+}
+
+}  // namespace kmc
