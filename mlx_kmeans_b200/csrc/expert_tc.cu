@@ -1,0 +1,502 @@
+// expert_tc.cu -- products of grouped rows with their expert's matrix on the tensor cores (tcgen05 + TMEM + TMA).
+//
+//   forward  y_p  = W_e x_row(p)              positions p of expert e: offsets[e] <= p < offsets[e + 1]
+//   dx       dx_p = W_e^T dy_p
+//   dW       dW_e = sum_p dy_p x_row(p)^T
+// 16-bit operands, float32 accumulation in TMEM, one rounding to 16 bits when a result is stored.
+//
+// The matrix is the MMA's A operand: 128 features are its M rows, and up to kCols positions its N columns.  N is a
+// run-time field of the instruction, so a group of any number of rows costs that number rounded up to 16 columns (not
+// to a tile of 128), and an expert's rows are cut into equal tiles rather than full ones and a rest.  For dx the same
+// matrix is read as its transpose (an MN-major A operand); dW takes both operands MN-major, with the positions as the
+// depth, so nothing is transposed in memory.  x's rows are gathered by TMA (tile::gather4, four row indices an
+// instruction): no permuted copy of x exists.  A position past the group's end, or a row outside x, is a row index past
+// the tensor: TMA fills it with zeros, so no other group's value (a NaN, say) enters a dW sum; in forward and dx a
+// neighbour's row can only reach columns that are not stored.
+//
+// Kernel layout (persistent, one CTA per SM): warp 0 loads (TMA), warp 1 issues the MMAs (64 deep a stage), warps 2-5
+// store the finished accumulator while the next one is computed (two accumulators in TMEM).  Every wait on an mbarrier
+// is bounded; on a timeout the CTA sets the error word, waits for its loads and MMAs in flight, and frees TMEM.
+#include <cuda.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+#include "experts.cuh"
+#include "kmc_internal.h"
+#include "tcgen05.cuh"
+
+namespace kmc {
+
+namespace {
+
+constexpr int kFeat = 128;                // features per tile (the MMA's M)
+constexpr int kDepth = 64;                // depth per stage: one 128-byte swizzle row of 16-bit elements
+constexpr int kTcThreads = 192;
+constexpr int kEpiThreads = 128;
+constexpr unsigned kFull = 0xffffffffu;
+
+struct TcArgs {
+    const int32_t* offsets;
+    const int32_t* rows;
+    int64_t x_rows;
+    int pairs, experts;
+    int feats;                            // M side in all: n (forward, dW), d (dx)
+    int cols;                             // dW: N side in all (d); otherwise unused
+    int depth;                            // forward: d, dx: n; dW: per expert
+    void* out;
+    int64_t ldo;                          // row length of out
+    int out_vec;                          // dW: rows of out start on 16-byte boundaries
+    int* error;
+};
+
+template <int COLS>
+struct TcSmem {
+    static constexpr int A = kFeat * kDepth * 2;
+    static constexpr int B = COLS * kDepth * 2;
+    static constexpr int STAGE = A + B;
+    static constexpr int BAR = 256;
+    static constexpr int EXPERTS = (kGroupMaxExperts + 1) * 4;
+    static constexpr int FREE = 227 * 1024 - BAR - EXPERTS - 1024;
+    static constexpr int NS = FREE / STAGE > 8 ? 8 : FREE / STAGE;
+    static constexpr int base = NS * STAGE + BAR + 1024;      // + the experts' tile counts
+    static_assert(NS >= 2 && 8 * (2 * NS + 5) + 8 <= BAR, "barrier block");
+};
+
+// Positions of expert e, with offsets that a caller made wrong kept inside the arrays.
+__device__ __forceinline__ void segment(const TcArgs& a, int e, int& begin, int& count) {
+    const int o0 = min(max(__ldg(a.offsets + e), 0), a.pairs), o1 = min(max(__ldg(a.offsets + e + 1), 0), a.pairs);
+    begin = o0;
+    count = o1 > o0 ? o1 - o0 : 0;
+}
+// Rows per tile of an expert with `count` rows: equal tiles of whole 16-column steps, at most COLS
+template <int COLS>
+__device__ __forceinline__ int tile_rows(int count) {
+    const int tiles = (count + COLS - 1) / COLS;
+    return tiles == 0 ? COLS : ((count + tiles - 1) / tiles + 15) / 16 * 16;
+}
+
+struct Tile {
+    int e, f0, c0;                        // expert, first feature, first column (dW)
+    int p0, p1;                           // positions: of the tile (forward, dx), of the expert (dW)
+    int ncols;                            // MMA columns (a multiple of 16)
+    int steps;                            // stages of depth
+};
+
+// Walks the tiles of one CTA in order; `first[e]` = tiles of experts before e (per feature tile).
+template <int MODE, int COLS>
+struct Walk {
+    int e;
+    __device__ __forceinline__ Walk() : e(0) {}
+    __device__ __forceinline__ Tile at(const TcArgs& a, const int* first, int64_t t) {
+        Tile r;
+        const int ft = (a.feats + kFeat - 1) / kFeat;
+        const int j = (int)(t / ft);
+        r.f0 = (int)(t - (int64_t)j * ft) * kFeat;
+        while (j >= first[e + 1]) e++;
+        r.e = e;
+        int begin, count;
+        segment(a, e, begin, count);
+        if constexpr (MODE == kExpertDw) {
+            r.c0 = (j - first[e]) * COLS;
+            r.p0 = begin;
+            r.p1 = begin + count;
+            const int left = a.cols - r.c0;
+            r.ncols = min((left + 15) / 16 * 16, COLS);
+            r.steps = (count + kDepth - 1) / kDepth;
+        } else {
+            const int size = tile_rows<COLS>(count);
+            r.c0 = 0;
+            r.p0 = begin + (j - first[e]) * size;
+            r.p1 = min(r.p0 + size, begin + count);
+            r.ncols = (r.p1 - r.p0 + 15) / 16 * 16;
+            r.steps = (a.depth + kDepth - 1) / kDepth;
+        }
+        return r;
+    }
+};
+
+// Row of x that position p reads, for TMA: x_rows (past the tensor: zeros) where there is none
+__device__ __forceinline__ int gather_row(const TcArgs& a, int p, int p1) {
+    if (p >= p1) return (int)a.x_rows;
+    const int r = a.rows ? __ldg(a.rows + p) : p;
+    return r < 0 || r >= a.x_rows ? (int)a.x_rows : r;
+}
+
+template <typename T, int MODE, int COLS, bool GATHER>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    k_expert_tc(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap ma_row,
+                const __grid_constant__ CUtensorMap mb, const __grid_constant__ CUtensorMap mb_row, TcArgs a) {
+    using S = TcSmem<COLS>;
+    constexpr int NS = S::NS;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    unsigned char* gbars = smem_raw + (base - raw) + NS * S::STAGE;
+    const uint32_t bars = base + NS * S::STAGE;
+    auto full = [&](int s) { return bars + 8u * s; };
+    auto empty = [&](int s) { return bars + 8u * (NS + s); };
+    auto accf = [&](int b) { return bars + 8u * (2 * NS + b); };
+    auto acce = [&](int b) { return bars + 8u * (2 * NS + 2 + b); };
+    const uint32_t drain = bars + 8u * (2 * NS + 4);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbars + 8 * (2 * NS + 5));
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(gbars + 8 * (2 * NS + 5) + 4);
+    int* first = reinterpret_cast<int*>(gbars + S::BAR);
+    __shared__ int part[kTcThreads / 32];
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < NS; s++) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), 1);
+        }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(accf(b), 1);
+            mbar_init(acce(b), kEpiThreads);
+        }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(2 * COLS));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    pdl_wait();
+    // first[e]: tiles of the experts before e, by a scan over per-thread runs of experts
+    {
+        const int run = (a.experts + kTcThreads - 1) / kTcThreads, e0 = min((int)threadIdx.x * run, a.experts);
+        const int e1 = min(e0 + run, a.experts);
+        auto tiles_of = [&](int e) {
+            int begin, count;
+            segment(a, e, begin, count);
+            if constexpr (MODE == kExpertDw) return (a.cols + COLS - 1) / COLS;
+            const int size = tile_rows<COLS>(count);
+            return (count + size - 1) / size;
+        };
+        int sum = 0;
+        for (int e = e0; e < e1; e++) sum += tiles_of(e);
+        int s = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(kFull, s, o);
+            if (lane >= o) s += up;
+        }
+        if (lane == 31) part[warp] = s;
+        __syncthreads();
+        int at = s - sum;
+        for (int w = 0; w < warp; w++) at += part[w];
+        for (int e = e0; e < e1; e++) {
+            first[e] = at;
+            at += tiles_of(e);
+        }
+        if (threadIdx.x == kTcThreads - 1) first[a.experts] = at;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int64_t tiles = (int64_t)first[a.experts] * ((a.feats + kFeat - 1) / kFeat);
+    Walk<MODE, COLS> walk;
+
+    if (warp == 0) {
+        // ---- loads: the whole warp, its lanes sharing the gathers of a stage
+        int stage = 0;
+        uint32_t phase = 0;
+        int64_t issued = 0;
+        bool ok = true;
+        for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+            const Tile w = walk.at(a, first, t);
+            int r0[4], r1[4];                              // rows of this lane's gathers (see below)
+            if constexpr (MODE != kExpertDw && GATHER) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    r0[i] = gather_row(a, w.p0 + lane * 4 + i, w.p1);
+                    if (COLS > 128) r1[i] = gather_row(a, w.p0 + (lane + 32) * 4 + i, w.p1);
+                }
+            }
+            if constexpr (MODE == kExpertDw && GATHER) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) r0[i] = gather_row(a, w.p0 + (lane & 15) * 4 + i, w.p1);
+            }
+            for (int kc = 0; kc < w.steps && ok; kc++) {
+                ok = __all_sync(kFull, mbar_wait(empty(stage), phase ^ 1u, abort_flag));
+                if (!ok) break;
+                const uint32_t sa = base + stage * S::STAGE, sb = sa + S::A, bar = full(stage);
+                if constexpr (MODE == kExpertDw) {
+                    // A: dy, two tiles of 64 features x 64 positions; B: x, up to four of 64 columns.  The last
+                    // positions of a group are gathered (zeros past its end), and so is x by its row indices.
+                    const int k0 = w.p0 + kc * kDepth;
+                    const bool tail = k0 + kDepth > w.p1;
+                    const int na = a.feats - w.f0 > 64 ? 2 : 1, nb = min((w.ncols + 63) / 64, COLS / 64);
+                    if (lane == 0) mbar_expect_tx(bar, (uint32_t)(na + nb) * 8192u);
+                    __syncwarp();
+                    if (!tail) {
+                        if (lane < na) tma_load_2d(sa + lane * 8192, &ma, w.f0 + lane * 64, k0, bar);
+                    } else {
+                        const int g = (lane & 15) * 4, h = lane >> 4;
+                        int q[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) q[i] = k0 + g + i < w.p1 ? k0 + g + i : a.pairs;
+                        if (h < na) tma_gather4(sa + h * 8192 + g * 128, &ma_row, w.f0 + h * 64, q, bar);
+                    }
+                    if (GATHER || tail) {
+                        const int g = (lane & 15) * 4;
+                        if constexpr (!GATHER) {
+#pragma unroll
+                            for (int i = 0; i < 4; i++) r0[i] = gather_row(a, k0 + g + i, w.p1);
+                        }
+                        for (int h = lane >> 4; h < nb; h += 2)
+                            tma_gather4(sb + h * 8192 + g * 128, &mb_row, w.c0 + h * 64, r0, bar);
+                        if constexpr (GATHER) {            // the next stage's rows, in flight meanwhile
+#pragma unroll
+                            for (int i = 0; i < 4; i++) r0[i] = gather_row(a, k0 + kDepth + g + i, w.p1);
+                        }
+                    } else {
+                        if (lane < nb) tma_load_2d(sb + lane * 8192, &mb, w.c0 + lane * 64, k0, bar);
+                    }
+                } else {
+                    const int nb = GATHER ? w.ncols / 4 : (w.ncols + 31) / 32;
+                    if (lane == 0) {
+                        mbar_expect_tx(bar, (uint32_t)(S::A + nb * (GATHER ? 512 : 4096)));
+                        if constexpr (MODE == kExpertForward) {        // 128 features x 64 deep
+                            tma_load_3d(sa, &ma, kc * kDepth, w.f0, w.e, bar);
+                        } else {                                       // two tiles of 64 deep x 64 features
+                            tma_load_3d(sa, &ma, w.f0, kc * kDepth, w.e, bar);
+                            tma_load_3d(sa + 8192, &ma, w.f0 + 64, kc * kDepth, w.e, bar);
+                        }
+                    }
+                    __syncwarp();
+                    if constexpr (GATHER) {
+                        if (lane < nb) tma_gather4(sb + lane * 512, &mb_row, kc * kDepth, r0, bar);
+                        if (COLS > 128 && lane + 32 < nb) tma_gather4(sb + (lane + 32) * 512, &mb_row, kc * kDepth, r1, bar);
+                    } else {
+                        if (lane < nb) tma_load_2d(sb + lane * 4096, &mb, kc * kDepth, w.p0 + lane * 32, bar);
+                    }
+                }
+                issued++;
+                if (++stage == NS) { stage = 0; phase ^= 1u; }
+            }
+        }
+        if (!ok) {                                         // a timeout: the loads in flight land before the CTA ends
+            for (int i = 0; i < NS && i < issued; i++) {
+                if (--stage < 0) { stage = NS - 1; phase ^= 1u; }
+                for (uint32_t n = 0; n < kSpinLimit && !mbar_try(full(stage), phase); n++) {}
+            }
+        }
+    } else if (warp == 1) {
+        // ---- MMA issuer
+        if (lane == 0) {
+            constexpr uint32_t type = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+            constexpr uint32_t amn = MODE != kExpertForward, bmn = MODE == kExpertDw;
+            constexpr uint32_t idesc0 = (1u << 4) | (type << 7) | (type << 10) | (amn << 15) | (bmn << 16) |
+                                        ((uint32_t)(kFeat >> 4) << 24);
+            int stage = 0;
+            uint32_t phase = 0, abuf = 0, aphase = 0;
+            bool ok = true;
+            for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+                const Tile w = walk.at(a, first, t);
+                if (w.steps == 0) continue;                // dW of an expert with no rows: nothing to add up
+                ok = mbar_wait(acce(abuf), aphase ^ 1u, abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t d_tmem = tmem + abuf * COLS;
+                const uint32_t idesc = idesc0 | ((uint32_t)(w.ncols >> 3) << 17);
+                const int deep = MODE == kExpertDw ? w.p1 - w.p0 : a.depth;
+                for (int kc = 0; kc < w.steps && ok; kc++) {
+                    ok = mbar_wait(full(stage), phase, abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t sa = base + stage * S::STAGE, sb = sa + S::A;
+                    const uint64_t da = amn ? sw128_desc_mn(sa, 8192) : sw128_desc(sa);
+                    const uint64_t db = bmn ? sw128_desc_mn(sb, 8192) : sw128_desc(sb);
+#pragma unroll
+                    for (int kk = 0; kk < kDepth / 16; kk++) {     // 16 deep: 32 B of a K-major row, 16 MN-major rows
+                        if (kc * kDepth + kk * 16 < deep)
+                            mma_f16(d_tmem, da + ((amn ? kk * 2048 : kk * 32) >> 4), db + ((bmn ? kk * 2048 : kk * 32) >> 4),
+                                    idesc, (kc | kk) != 0);
+                    }
+                    mma_commit(empty(stage));
+                    if (++stage == NS) { stage = 0; phase ^= 1u; }
+                }
+                if (!ok) break;
+                mma_commit(accf(abuf));
+                abuf ^= 1u;
+                if (abuf == 0) aphase ^= 1u;
+            }
+            if (!ok) {                                     // a timeout: the MMAs issued so far end before TMEM is freed
+                mma_commit(drain);
+                for (uint32_t n = 0; n < kSpinLimit && !mbar_try(drain, 0); n++) {}
+            }
+        }
+    } else {
+        // ---- epilogue: warp w reads TMEM lane quarter w % 4 (features), 32 columns at a time
+        const int q = warp & 3;
+        const uint32_t lane_base = tmem + ((uint32_t)(32 * q) << 16);
+        T* out = static_cast<T*>(a.out);
+        uint32_t abuf = 0, aphase = 0;
+        bool ok = true;
+        if constexpr (MODE != kExpertDw) {                 // rows past the last group: zeros
+            const int64_t taken = min(max(__ldg(a.offsets + a.experts), 0), a.pairs);
+            for (int64_t i = taken * a.ldo + (int64_t)blockIdx.x * kEpiThreads + threadIdx.x - 64;
+                 i < a.pairs * a.ldo; i += (int64_t)gridDim.x * kEpiThreads)
+                out[i] = Elem<T>::from(0.0f);
+        }
+        for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+            const Tile w = walk.at(a, first, t);
+            if (w.steps > 0) {
+                ok = mbar_wait(accf(abuf), aphase, abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+            }
+            const int f = w.f0 + 32 * q + lane;
+            for (int c = 0; c < w.ncols; c += 32) {
+                float v[32];
+                if (w.steps > 0) {
+                    tmem_ld32(lane_base + abuf * COLS + c, v);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; j++) v[j] = 0.0f;
+                }
+                if constexpr (MODE == kExpertDw) {
+                    if (f < a.feats) {
+                        T* dst = out + ((int64_t)w.e * a.feats + f) * a.ldo + w.c0 + c;
+                        const int left = a.cols - w.c0 - c;
+#pragma unroll
+                        for (int g = 0; g < 4; g++) {
+                            if (a.out_vec && g * 8 + 8 <= left) {
+                                Pack<T, 8> p;
+#pragma unroll
+                                for (int j = 0; j < 8; j++) p.v[j] = Elem<T>::from(v[g * 8 + j]);
+                                *reinterpret_cast<Pack<T, 8>*>(dst + g * 8) = p;
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < 8; j++)
+                                    if (g * 8 + j < left) dst[g * 8 + j] = Elem<T>::from(v[g * 8 + j]);
+                            }
+                        }
+                    }
+                } else {
+                    if (f < a.feats) {
+                        const int left = w.p1 - w.p0 - c;
+                        T* dst = out + (int64_t)(w.p0 + c) * a.ldo + f;
+#pragma unroll
+                        for (int j = 0; j < 32; j++)
+                            if (j < left) dst[j * a.ldo] = Elem<T>::from(v[j]);
+                    }
+                }
+            }
+            if (w.steps > 0) {
+                tc_fence_before();
+                mbar_arrive(acce(abuf));
+                abuf ^= 1u;
+                if (abuf == 0) aphase ^= 1u;
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * COLS));
+    }
+    if (threadIdx.x == 0 && *abort_flag) atomicExch(a.error, 1);
+}
+
+// ---------------------------------------------------------------- host side
+
+// rows x cols (x planes) of 16-bit elements, rows ld apart; box of 64 columns x box_rows, 128-byte swizzle, zeros
+// outside
+bool make_map(CUtensorMap* m, int dtype, const void* base, int64_t cols, int64_t rows, int64_t planes, int64_t ld, int box_rows) {
+    auto fn = tensor_map_encode();
+    if (!fn) return false;
+    cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)(planes > 0 ? planes : 1)};
+    cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)ld * rows * 2};
+    cuuint32_t box[3] = {(cuuint32_t)kDepth, (cuuint32_t)box_rows, 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = fn(m, dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                    planes > 0 ? 3 : 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS;
+}
+
+template <typename T, int MODE, int COLS, bool GATHER>
+cudaError_t run_tc(const CUtensorMap (&m)[4], const TcArgs& a, cudaStream_t st) {
+    auto kern = k_expert_tc<T, MODE, COLS, GATHER>;
+    const size_t smem = TcSmem<COLS>::base + (size_t)(a.experts + 1) * 4;
+    static unsigned long long configured = 0;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!(configured >> (dev & 63) & 1ull)) {
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             TcSmem<COLS>::base + TcSmem<COLS>::EXPERTS);
+        if (e != cudaSuccess) return e;
+        configured |= 1ull << (dev & 63);
+    }
+    return launch_pdl(kern, dim3(num_sms()), dim3(kTcThreads), smem, st, m[0], m[1], m[2], m[3], a);
+}
+
+template <typename T>
+cudaError_t run_kind(const ExpertCall& c, const Operands& o, cudaStream_t st) {
+    CUtensorMap m[4];
+    TcArgs a = {};
+    a.offsets = c.offsets;
+    a.rows = c.rows;
+    a.pairs = (int)c.pairs;
+    a.experts = c.experts;
+    a.error = c.error;
+    bool ok;
+    // positions per tile: 64 where the experts' mean is below that (a stage is then 24 KB and eight are in flight)
+    const bool few = c.pairs <= (int64_t)c.experts * 64;
+    switch (c.kind) {
+        case kExpertForward:
+            a.x_rows = c.x_rows;
+            a.feats = c.n;
+            a.depth = c.d;
+            a.out = c.y;
+            a.ldo = c.n;
+            ok = make_map(&m[0], c.dtype, o.w, c.d, c.n, c.experts, o.ldw, kFeat) &&
+                 make_map(&m[2], c.dtype, o.x, c.d, c.x_rows, 0, o.ldx, 32) &&
+                 make_map(&m[3], c.dtype, o.x, c.d, c.x_rows, 0, o.ldx, 1);
+            m[1] = m[0];
+            if (!ok) return cudaErrorInvalidValue;
+            if (c.rows) return few ? run_tc<T, kExpertForward, 64, true>(m, a, st) : run_tc<T, kExpertForward, 256, true>(m, a, st);
+            return few ? run_tc<T, kExpertForward, 64, false>(m, a, st) : run_tc<T, kExpertForward, 256, false>(m, a, st);
+        case kExpertDx:
+            a.rows = nullptr;
+            a.x_rows = c.pairs;
+            a.feats = c.d;
+            a.depth = c.n;
+            a.out = c.dx;
+            a.ldo = c.d;
+            ok = make_map(&m[0], c.dtype, o.w, c.d, c.n, c.experts, o.ldw, kDepth) &&
+                 make_map(&m[2], c.dtype, o.dy, c.n, c.pairs, 0, o.lddy, 32);
+            m[1] = m[0];
+            m[3] = m[2];
+            if (!ok) return cudaErrorInvalidValue;
+            return few ? run_tc<T, kExpertDx, 64, false>(m, a, st) : run_tc<T, kExpertDx, 256, false>(m, a, st);
+        default:
+            a.x_rows = c.x_rows;
+            a.feats = c.n;
+            a.cols = c.d;
+            a.out = c.dw;
+            a.ldo = c.d;
+            a.out_vec = c.d % 8 == 0 && reinterpret_cast<uintptr_t>(c.dw) % 16 == 0;
+            ok = make_map(&m[0], c.dtype, o.dy, c.n, c.pairs, 0, o.lddy, kDepth) &&
+                 make_map(&m[1], c.dtype, o.dy, c.n, c.pairs, 0, o.lddy, 1) &&
+                 make_map(&m[2], c.dtype, o.x, c.d, c.x_rows, 0, o.ldx, kDepth) &&
+                 make_map(&m[3], c.dtype, o.x, c.d, c.x_rows, 0, o.ldx, 1);
+            if (!ok) return cudaErrorInvalidValue;
+            return c.rows ? run_tc<T, kExpertDw, 256, true>(m, a, st) : run_tc<T, kExpertDw, 256, false>(m, a, st);
+    }
+}
+
+}  // namespace
+
+cudaError_t launch_expert_tc(const ExpertCall& c, const Operands& o, cudaStream_t st) {
+    return c.dtype == 1 ? run_kind<__nv_bfloat16>(c, o, st) : run_kind<__half>(c, o, st);
+}
+
+}  // namespace kmc

@@ -267,7 +267,13 @@ struct ExpertCall {
     void* ws;                 // expert_bytes(call) bytes
     int* error;               // set to 1 by a kernel that gave up on a barrier
 };
-size_t expert_bytes(const ExpertCall& c);
+size_t expert_bytes(const ExpertCall& c);   // by the operands' pointers, sizes and row strides
 cudaError_t launch_expert(const ExpertCall& c, cudaStream_t st);
+// the 16-bit operands as the tensor-core kernel reads them: 16-byte aligned, rows a multiple of 8 elements apart
+struct Operands {
+    const void *x, *w, *dy;
+    int64_t ldx, ldw, lddy;
+};
+cudaError_t launch_expert_tc(const ExpertCall& c, const Operands& o, cudaStream_t st);
 
 }  // namespace kmc
