@@ -371,11 +371,12 @@ int kmc_group_rows(const int32_t *ids, int64_t rows, int choices, int experts, i
  * grouped (x_rows = pairs).  Positions past offsets[experts] get zeros.  dtype KMC_BF16 or KMC_F16 throughout.
  * kmc_expert_matmul_dx: dx (pairs x d) = W_e^T dy (pairs x n), by position (sum a row's positions with kmc_combine).
  * kmc_expert_matmul_dw: dW (experts x n x d) = sum over an expert's positions of dy x^T; 0 for an expert with none.
- * workspace: kmc_expert_bytes bytes for the call's operands (NULL for one it does not take), 256-byte aligned; 0 where
- * each starts on 16 bytes with rows a multiple of 8 elements apart, otherwise room for padded copies.  error (device int32, set to 0 once by the
+ * workspace: kmc_expert_bytes bytes for the call's operands (NULL for one it does not take), 256-byte aligned: room for
+ * x in grouped order where that is read faster, and for padded copies of operands that do not start on 16 bytes or have
+ * rows that are not a multiple of 8 elements apart; may be 0.  error (device int32, set to 0 once by the
  * caller): 1 once a kernel gave up waiting on a barrier, its output then incomplete. */
-size_t kmc_expert_bytes(const void *x, int64_t x_rows, int64_t ldx, const void *w, const void *dy, int64_t pairs,
-                        int experts, int n, int d);
+size_t kmc_expert_bytes(const void *x, int64_t x_rows, int64_t ldx, const int32_t *group_row, const void *w,
+                        const void *dy, int64_t pairs, int experts, int n, int d);
 int kmc_expert_matmul(const void *x, int64_t x_rows, int64_t ldx, const int32_t *group_row, const void *w,
                       const int32_t *offsets, int64_t pairs, int experts, int n, int d, int dtype, void *y,
                       void *workspace, size_t ws_bytes, int32_t *error, void *stream);

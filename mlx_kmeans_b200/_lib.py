@@ -81,7 +81,7 @@ SIGNATURES = {
     "kmc_route_grad": (_int, [_vp, _vp, _int, _i64, _int, _i64, _vp, _int, _f, _u, _vp, _vp]),
     "kmc_group_bytes": (_sz, [_i64, _int]),
     "kmc_group_rows": (_int, [_vp, _i64, _int, _int, _vp, _vp, _vp, _vp, _sz, _vp]),
-    "kmc_expert_bytes": (_sz, [_vp, _i64, _i64, _vp, _vp, _i64, _int, _int, _int]),
+    "kmc_expert_bytes": (_sz, [_vp, _i64, _i64, _vp, _vp, _vp, _i64, _int, _int, _int]),
     "kmc_expert_matmul": (_int, [_vp, _i64, _i64, _vp, _vp, _vp, _i64, _int, _int, _int, _int, _vp, _vp, _sz, _vp,
                                  _vp]),
     "kmc_expert_matmul_dx": (_int, [_vp, _vp, _vp, _i64, _int, _int, _int, _int, _vp, _vp, _sz, _vp, _vp]),

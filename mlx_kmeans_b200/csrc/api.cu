@@ -980,13 +980,15 @@ int kmc_expert_matmul_dw(const void* dy, const void* x, int64_t x_rows, int64_t 
     return run_expert("kmc_expert_matmul_dw", c, ws_bytes, stream);
 }
 
-size_t kmc_expert_bytes(const void* x, int64_t x_rows, int64_t ldx, const void* w, const void* dy, int64_t pairs,
-                        int experts, int n, int d) {
+size_t kmc_expert_bytes(const void* x, int64_t x_rows, int64_t ldx, const int32_t* group_row, const void* w,
+                        const void* dy, int64_t pairs, int experts, int n, int d) {
     if (x_rows < 0 || pairs < 0 || experts < 1 || n < 1 || d < 1) return 0;
     ExpertCall c = {};
+    c.kind = !dy ? kExpertForward : w ? kExpertDx : kExpertDw;
     c.x = x;
     c.x_rows = x_rows;
     c.ldx = ldx;
+    c.rows = group_row;
     c.w = w;
     c.dy = dy;
     c.pairs = pairs;

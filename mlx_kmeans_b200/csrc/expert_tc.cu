@@ -5,18 +5,23 @@
 //   dW       dW_e = sum_p dy_p x_row(p)^T
 // 16-bit operands, float32 accumulation in TMEM, one rounding to 16 bits when a result is stored.
 //
-// The matrix is the MMA's A operand: 128 features are its M rows, and up to kCols positions its N columns.  N is a
-// run-time field of the instruction, so a group of any number of rows costs that number rounded up to 16 columns (not
-// to a tile of 128), and an expert's rows are cut into equal tiles rather than full ones and a rest.  For dx the same
-// matrix is read as its transpose (an MN-major A operand); dW takes both operands MN-major, with the positions as the
-// depth, so nothing is transposed in memory.  x's rows are gathered by TMA (tile::gather4, four row indices an
-// instruction): no permuted copy of x exists.  A position past the group's end, or a row outside x, is a row index past
-// the tensor: TMA fills it with zeros, so no other group's value (a NaN, say) enters a dW sum; in forward and dx a
-// neighbour's row can only reach columns that are not stored.
+// The matrix is the MMA's A operand: features are its M rows, and up to COLS positions its N columns.  N is a run-time
+// field of the instruction, so a group of any number of rows costs that number rounded up to 16 (32 for a pair of
+// CTAs), not to a tile of 128, and an expert's rows are cut into equal tiles rather than full ones and a rest.  For dx
+// the same matrix is read as its transpose (an MN-major A operand); dW takes both operands MN-major, with the positions
+// as the depth, so nothing is transposed in memory.
 //
-// Kernel layout (persistent, one CTA per SM): warp 0 loads (TMA), warp 1 issues the MMAs (64 deep a stage), warps 2-5
-// store the finished accumulator while the next one is computed (two accumulators in TMEM).  Every wait on an mbarrier
-// is bounded; on a timeout the CTA sets the error word, waits for its loads and MMAs in flight, and frees TMEM.
+// PAIR: two CTAs of a cluster share each MMA (cta_group::2): 256 features x up to 256 positions, each CTA holding 128
+// of the features and half of the positions, so a stage of 64 deep is 32 KB a CTA instead of 48 KB for the same work
+// (what the L2 can deliver bounds the single-CTA tile).  GATHER (few rows an expert): x's rows are read in place by
+// their indices (tile::gather4, four rows an instruction).  A row index past the tensor is filled with zeros by TMA:
+// positions past a group's end in dW are loaded that way, so no other group's value (a NaN, say) enters the sum; in
+// forward and dx a neighbour's row can only reach columns that are not stored.
+//
+// Kernel layout (persistent, one CTA per SM): warp 0 loads (TMA), warp 1 issues the MMAs (64 deep a stage; in a pair
+// the leader's alone), warps 2-5 store the finished accumulator while the next one is computed (two accumulators in
+// TMEM).  Every wait on an mbarrier is bounded; on a timeout the CTA sets the error word, waits for its loads and MMAs
+// in flight, and frees TMEM.
 #include <cuda.h>
 
 #include <type_traits>
@@ -30,8 +35,9 @@ namespace kmc {
 
 namespace {
 
-constexpr int kFeat = 128;                // features per tile (the MMA's M)
+constexpr int kFeat = 128;                // features per CTA and tile (the MMA's M, or half of it)
 constexpr int kDepth = 64;                // depth per stage: one 128-byte swizzle row of 16-bit elements
+constexpr int kBox = 64 * kDepth * 2;     // 64 x 64 elements
 constexpr int kTcThreads = 192;
 constexpr int kEpiThreads = 128;
 constexpr unsigned kFull = 0xffffffffu;
@@ -50,14 +56,15 @@ struct TcArgs {
     int* error;
 };
 
-template <int COLS>
+template <int COLS, bool PAIR>
 struct TcSmem {
+    static constexpr int MINE = PAIR ? COLS / 2 : COLS;       // columns whose operand this CTA holds
     static constexpr int A = kFeat * kDepth * 2;
-    static constexpr int B = COLS * kDepth * 2;
+    static constexpr int B = MINE * kDepth * 2;
     static constexpr int STAGE = A + B;
     static constexpr int BAR = 256;
     static constexpr int EXPERTS = (kGroupMaxExperts + 1) * 4;
-    static constexpr int FREE = 227 * 1024 - BAR - EXPERTS - 1024;
+    static constexpr int FREE = 227 * 1024 - BAR - EXPERTS - 2048;   // 1 KB to align, 1 KB of static arrays
     static constexpr int NS = FREE / STAGE > 8 ? 8 : FREE / STAGE;
     static constexpr int base = NS * STAGE + BAR + 1024;      // + the experts' tile counts
     static_assert(NS >= 2 && 8 * (2 * NS + 5) + 8 <= BAR, "barrier block");
@@ -69,30 +76,38 @@ __device__ __forceinline__ void segment(const TcArgs& a, int e, int& begin, int&
     begin = o0;
     count = o1 > o0 ? o1 - o0 : 0;
 }
-// Rows per tile of an expert with `count` rows: equal tiles of whole 16-column steps, at most COLS
-template <int COLS>
-__device__ __forceinline__ int tile_rows(int count) {
-    const int tiles = (count + COLS - 1) / COLS;
-    return tiles == 0 ? COLS : ((count + tiles - 1) / tiles + 15) / 16 * 16;
-}
 
 struct Tile {
     int e, f0, c0;                        // expert, first feature, first column (dW)
     int p0, p1;                           // positions: of the tile (forward, dx), of the expert (dW)
-    int ncols;                            // MMA columns (a multiple of 16)
+    int ncols;                            // MMA columns (a multiple of Shape::STEP)
     int steps;                            // stages of depth
 };
 
-// Walks the tiles of one CTA in order; `first[e]` = tiles of experts before e (per feature tile).
-template <int MODE, int COLS>
-struct Walk {
-    int e;
-    __device__ __forceinline__ Walk() : e(0) {}
-    __device__ __forceinline__ Tile at(const TcArgs& a, const int* first, int64_t t) {
+template <int MODE, int COLS, bool PAIR>
+struct Shape {
+    static constexpr int FEATS = PAIR ? 2 * kFeat : kFeat;    // features per tile
+    static constexpr int STEP = PAIR ? 32 : 16;               // granularity of the MMA's N
+
+    static __device__ __forceinline__ int feature_tiles(const TcArgs& a) { return (a.feats + FEATS - 1) / FEATS; }
+    // Rows per tile of an expert with `count` rows: equal tiles of whole STEPs, at most COLS
+    static __device__ __forceinline__ int rows(int count) {
+        const int tiles = (count + COLS - 1) / COLS;
+        return tiles == 0 ? COLS : ((count + tiles - 1) / tiles + STEP - 1) / STEP * STEP;
+    }
+    // Tiles of expert e per feature tile
+    static __device__ __forceinline__ int tiles(const TcArgs& a, int e) {
+        if constexpr (MODE == kExpertDw) return (a.cols + COLS - 1) / COLS;
+        int begin, count;
+        segment(a, e, begin, count);
+        const int size = rows(count);
+        return (count + size - 1) / size;
+    }
+    // Tile t; `e` walks up with t, first[e] = tiles of the experts before e.
+    static __device__ __forceinline__ Tile at(const TcArgs& a, const int* first, int64_t t, int& e) {
         Tile r;
-        const int ft = (a.feats + kFeat - 1) / kFeat;
-        const int j = (int)(t / ft);
-        r.f0 = (int)(t - (int64_t)j * ft) * kFeat;
+        const int ft = feature_tiles(a), j = (int)(t / ft);
+        r.f0 = (int)(t - (int64_t)j * ft) * FEATS;
         while (j >= first[e + 1]) e++;
         r.e = e;
         int begin, count;
@@ -101,15 +116,14 @@ struct Walk {
             r.c0 = (j - first[e]) * COLS;
             r.p0 = begin;
             r.p1 = begin + count;
-            const int left = a.cols - r.c0;
-            r.ncols = min((left + 15) / 16 * 16, COLS);
+            r.ncols = min((a.cols - r.c0 + STEP - 1) / STEP * STEP, COLS);
             r.steps = (count + kDepth - 1) / kDepth;
         } else {
-            const int size = tile_rows<COLS>(count);
+            const int size = rows(count);
             r.c0 = 0;
             r.p0 = begin + (j - first[e]) * size;
             r.p1 = min(r.p0 + size, begin + count);
-            r.ncols = (r.p1 - r.p0 + 15) / 16 * 16;
+            r.ncols = (r.p1 - r.p0 + STEP - 1) / STEP * STEP;
             r.steps = (a.depth + kDepth - 1) / kDepth;
         }
         return r;
@@ -123,12 +137,31 @@ __device__ __forceinline__ int gather_row(const TcArgs& a, int p, int p1) {
     return r < 0 || r >= a.x_rows ? (int)a.x_rows : r;
 }
 
-template <typename T, int MODE, int COLS, bool GATHER>
+template <bool PAIR>
+__device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* m, int x, int y, uint32_t bar) {
+    if constexpr (PAIR) tma_load_2d_pair(dst, m, x, y, bar);
+    else tma_load_2d(dst, m, x, y, bar);
+}
+template <bool PAIR>
+__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* m, int x, int y, int z, uint32_t bar) {
+    if constexpr (PAIR) tma_load_3d_pair(dst, m, x, y, z, bar);
+    else tma_load_3d(dst, m, x, y, z, bar);
+}
+template <bool PAIR>
+__device__ __forceinline__ void gather4(uint32_t dst, const CUtensorMap* m, int x, const int (&r)[4], uint32_t bar) {
+    if constexpr (PAIR) tma_gather4_pair(dst, m, x, r, bar);
+    else tma_gather4(dst, m, x, r, bar);
+}
+
+template <typename T, int MODE, int COLS, bool GATHER, bool PAIR>
 __global__ void __launch_bounds__(kTcThreads, 1)
     k_expert_tc(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap ma_row,
                 const __grid_constant__ CUtensorMap mb, const __grid_constant__ CUtensorMap mb_row, TcArgs a) {
-    using S = TcSmem<COLS>;
+    static_assert(!GATHER || (MODE == kExpertForward && !PAIR && COLS <= 128), "gathers: one per lane and stage");
+    using S = TcSmem<COLS, PAIR>;
+    using Sh = Shape<MODE, COLS, PAIR>;
     constexpr int NS = S::NS;
+    constexpr int CTAS = PAIR ? 2 : 1;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
@@ -145,38 +178,38 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     __shared__ int part[kTcThreads / 32];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = PAIR ? (int)cluster_rank() : 0;       // 0: the pair's leader
     if (threadIdx.x == 0) {
         for (int s = 0; s < NS; s++) {
-            mbar_init(full(s), 1);
+            mbar_init(full(s), 1);                         // the leader's load warp; both CTAs' bytes count on it
             mbar_init(empty(s), 1);
         }
         for (int b = 0; b < 2; b++) {
             mbar_init(accf(b), 1);
-            mbar_init(acce(b), kEpiThreads);
+            mbar_init(acce(b), CTAS * kEpiThreads / 32);   // a lane of each epilogue warp, of both CTAs
         }
         mbar_init(drain, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                     "r"(2 * COLS));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                         "r"(2 * COLS));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                         "r"(2 * COLS));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        }
     }
     pdl_wait();
     // first[e]: tiles of the experts before e, by a scan over per-thread runs of experts
     {
         const int run = (a.experts + kTcThreads - 1) / kTcThreads, e0 = min((int)threadIdx.x * run, a.experts);
         const int e1 = min(e0 + run, a.experts);
-        auto tiles_of = [&](int e) {
-            int begin, count;
-            segment(a, e, begin, count);
-            if constexpr (MODE == kExpertDw) return (a.cols + COLS - 1) / COLS;
-            const int size = tile_rows<COLS>(count);
-            return (count + size - 1) / size;
-        };
         int sum = 0;
-        for (int e = e0; e < e1; e++) sum += tiles_of(e);
+        for (int e = e0; e < e1; e++) sum += Sh::tiles(a, e);
         int s = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -189,114 +222,101 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int w = 0; w < warp; w++) at += part[w];
         for (int e = e0; e < e1; e++) {
             first[e] = at;
-            at += tiles_of(e);
+            at += Sh::tiles(a, e);
         }
         if (threadIdx.x == kTcThreads - 1) first[a.experts] = at;
     }
     tc_fence_before();
-    __syncthreads();
+    if constexpr (PAIR) cluster_sync();
+    else __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const int64_t tiles = (int64_t)first[a.experts] * ((a.feats + kFeat - 1) / kFeat);
-    Walk<MODE, COLS> walk;
+    const int64_t tiles = (int64_t)first[a.experts] * Sh::feature_tiles(a);
+    const int64_t t0 = blockIdx.x / CTAS, dt = gridDim.x / CTAS;
+    int e = 0;
 
     if (warp == 0) {
-        // ---- loads: the whole warp, its lanes sharing the gathers of a stage
+        // ---- loads: the whole warp, its lanes sharing the copies of a stage
         int stage = 0;
         uint32_t phase = 0;
         int64_t issued = 0;
         bool ok = true;
-        for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-            const Tile w = walk.at(a, first, t);
-            int r0[4], r1[4];                              // rows of this lane's gathers (see below)
-            if constexpr (MODE != kExpertDw && GATHER) {
+        for (int64_t t = t0; t < tiles && ok; t += dt) {
+            const Tile w = Sh::at(a, first, t, e);
+            const int f0 = w.f0 + rank * kFeat;
+            const int half = w.ncols / CTAS;               // columns of this CTA's operand
+            int r[4];                                      // rows of this lane's gather
+            if constexpr (GATHER) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    r0[i] = gather_row(a, w.p0 + lane * 4 + i, w.p1);
-                    if (COLS > 128) r1[i] = gather_row(a, w.p0 + (lane + 32) * 4 + i, w.p1);
-                }
-            }
-            if constexpr (MODE == kExpertDw && GATHER) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) r0[i] = gather_row(a, w.p0 + (lane & 15) * 4 + i, w.p1);
+                for (int i = 0; i < 4; i++) r[i] = gather_row(a, w.p0 + lane * 4 + i, w.p1);
             }
             for (int kc = 0; kc < w.steps && ok; kc++) {
                 ok = __all_sync(kFull, mbar_wait(empty(stage), phase ^ 1u, abort_flag));
                 if (!ok) break;
-                const uint32_t sa = base + stage * S::STAGE, sb = sa + S::A, bar = full(stage);
+                const uint32_t sa = base + stage * S::STAGE, sb = sa + S::A;
+                const uint32_t bar = PAIR ? cluster_addr(full(stage), 0) : full(stage);
                 if constexpr (MODE == kExpertDw) {
-                    // A: dy, two tiles of 64 features x 64 positions; B: x, up to four of 64 columns.  The last
-                    // positions of a group are gathered (zeros past its end), and so is x by its row indices.
-                    const int k0 = w.p0 + kc * kDepth;
-                    const bool tail = k0 + kDepth > w.p1;
-                    const int na = a.feats - w.f0 > 64 ? 2 : 1, nb = min((w.ncols + 63) / 64, COLS / 64);
-                    if (lane == 0) mbar_expect_tx(bar, (uint32_t)(na + nb) * 8192u);
+                    // A: dy, two boxes of 64 features x 64 positions; B: x, boxes of 64 columns.  The last positions of
+                    // a group are gathered, zeros past its end.
+                    const int k0 = w.p0 + kc * kDepth, nb = (half + 63) / 64, c0 = w.c0 + rank * half;
+                    if (lane == 0 && rank == 0) mbar_expect_tx(full(stage), (uint32_t)(CTAS * (2 + nb)) * kBox);
                     __syncwarp();
-                    if (!tail) {
-                        if (lane < na) tma_load_2d(sa + lane * 8192, &ma, w.f0 + lane * 64, k0, bar);
+                    if (k0 + kDepth <= w.p1) {
+                        if (lane < 2) load_2d<PAIR>(sa + lane * kBox, &ma, f0 + lane * 64, k0, bar);
+                        else if (lane < 2 + nb) load_2d<PAIR>(sb + (lane - 2) * kBox, &mb, c0 + (lane - 2) * 64, k0, bar);
                     } else {
-                        const int g = (lane & 15) * 4, h = lane >> 4;
-                        int q[4];
-#pragma unroll
-                        for (int i = 0; i < 4; i++) q[i] = k0 + g + i < w.p1 ? k0 + g + i : a.pairs;
-                        if (h < na) tma_gather4(sa + h * 8192 + g * 128, &ma_row, w.f0 + h * 64, q, bar);
-                    }
-                    if (GATHER || tail) {
                         const int g = (lane & 15) * 4;
-                        if constexpr (!GATHER) {
+                        int q[4], x[4];
 #pragma unroll
-                            for (int i = 0; i < 4; i++) r0[i] = gather_row(a, k0 + g + i, w.p1);
+                        for (int i = 0; i < 4; i++) {
+                            q[i] = k0 + g + i < w.p1 ? k0 + g + i : a.pairs;
+                            x[i] = gather_row(a, k0 + g + i, w.p1);
                         }
+                        gather4<PAIR>(sa + (lane >> 4) * kBox + g * 128, &ma_row, f0 + (lane >> 4) * 64, q, bar);
                         for (int h = lane >> 4; h < nb; h += 2)
-                            tma_gather4(sb + h * 8192 + g * 128, &mb_row, w.c0 + h * 64, r0, bar);
-                        if constexpr (GATHER) {            // the next stage's rows, in flight meanwhile
-#pragma unroll
-                            for (int i = 0; i < 4; i++) r0[i] = gather_row(a, k0 + kDepth + g + i, w.p1);
-                        }
-                    } else {
-                        if (lane < nb) tma_load_2d(sb + lane * 8192, &mb, w.c0 + lane * 64, k0, bar);
+                            gather4<PAIR>(sb + h * kBox + g * 128, &mb_row, c0 + h * 64, x, bar);
                     }
                 } else {
-                    const int nb = GATHER ? w.ncols / 4 : (w.ncols + 31) / 32;
+                    const int nb = GATHER ? half / 4 : (half + 31) / 32;
                     if (lane == 0) {
-                        mbar_expect_tx(bar, (uint32_t)(S::A + nb * (GATHER ? 512 : 4096)));
+                        if (rank == 0) mbar_expect_tx(full(stage), (uint32_t)(CTAS * (S::A + nb * (GATHER ? 512 : 4096))));
                         if constexpr (MODE == kExpertForward) {        // 128 features x 64 deep
-                            tma_load_3d(sa, &ma, kc * kDepth, w.f0, w.e, bar);
-                        } else {                                       // two tiles of 64 deep x 64 features
-                            tma_load_3d(sa, &ma, w.f0, kc * kDepth, w.e, bar);
-                            tma_load_3d(sa + 8192, &ma, w.f0 + 64, kc * kDepth, w.e, bar);
+                            load_3d<PAIR>(sa, &ma, kc * kDepth, f0, w.e, bar);
+                        } else {                                       // two boxes of 64 deep x 64 features
+                            load_3d<PAIR>(sa, &ma, f0, kc * kDepth, w.e, bar);
+                            load_3d<PAIR>(sa + kBox, &ma, f0 + 64, kc * kDepth, w.e, bar);
                         }
                     }
                     __syncwarp();
-                    if constexpr (GATHER) {
-                        if (lane < nb) tma_gather4(sb + lane * 512, &mb_row, kc * kDepth, r0, bar);
-                        if (COLS > 128 && lane + 32 < nb) tma_gather4(sb + (lane + 32) * 512, &mb_row, kc * kDepth, r1, bar);
-                    } else {
-                        if (lane < nb) tma_load_2d(sb + lane * 4096, &mb, kc * kDepth, w.p0 + lane * 32, bar);
+                    if (lane < nb) {
+                        if constexpr (GATHER) gather4<PAIR>(sb + lane * 512, &mb_row, kc * kDepth, r, bar);
+                        else load_2d<PAIR>(sb + lane * 4096, &mb, kc * kDepth, w.p0 + rank * half + lane * 32, bar);
                     }
                 }
                 issued++;
                 if (++stage == NS) { stage = 0; phase ^= 1u; }
             }
         }
-        if (!ok) {                                         // a timeout: the loads in flight land before the CTA ends
-            for (int i = 0; i < NS && i < issued; i++) {
-                if (--stage < 0) { stage = NS - 1; phase ^= 1u; }
-                for (uint32_t n = 0; n < kSpinLimit && !mbar_try(full(stage), phase); n++) {}
-            }
+        // the loads in flight have landed (a timeout) and both CTAs are done with every stage (a pair: the leader's
+        // MMAs read this CTA's stages and its commits arrive here) before the CTA ends
+        for (int i = 0; i < NS && i < issued; i++) {
+            if (--stage < 0) { stage = NS - 1; phase ^= 1u; }
+            const uint32_t bar = ok ? empty(stage) : full(stage);
+            if (PAIR ? (ok || rank == 0) : !ok)
+                for (uint32_t n = 0; n < kSpinLimit && !mbar_try(bar, phase); n++) {}
         }
     } else if (warp == 1) {
         // ---- MMA issuer
-        if (lane == 0) {
-            constexpr uint32_t type = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
             constexpr uint32_t amn = MODE != kExpertForward, bmn = MODE == kExpertDw;
             constexpr uint32_t idesc0 = (1u << 4) | (type << 7) | (type << 10) | (amn << 15) | (bmn << 16) |
-                                        ((uint32_t)(kFeat >> 4) << 24);
+                                        ((uint32_t)(Sh::FEATS >> 4) << 24);
             int stage = 0;
             uint32_t phase = 0, abuf = 0, aphase = 0;
             bool ok = true;
-            for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-                const Tile w = walk.at(a, first, t);
+            for (int64_t t = t0; t < tiles && ok; t += dt) {
+                const Tile w = Sh::at(a, first, t, e);
                 if (w.steps == 0) continue;                // dW of an expert with no rows: nothing to add up
                 ok = mbar_wait(acce(abuf), aphase ^ 1u, abort_flag);
                 if (!ok) break;
@@ -309,24 +329,29 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t sa = base + stage * S::STAGE, sb = sa + S::A;
-                    const uint64_t da = amn ? sw128_desc_mn(sa, 8192) : sw128_desc(sa);
-                    const uint64_t db = bmn ? sw128_desc_mn(sb, 8192) : sw128_desc(sb);
+                    const uint64_t da = amn ? sw128_desc_mn(sa, kBox) : sw128_desc(sa);
+                    const uint64_t db = bmn ? sw128_desc_mn(sb, kBox) : sw128_desc(sb);
 #pragma unroll
                     for (int kk = 0; kk < kDepth / 16; kk++) {     // 16 deep: 32 B of a K-major row, 16 MN-major rows
-                        if (kc * kDepth + kk * 16 < deep)
-                            mma_f16(d_tmem, da + ((amn ? kk * 2048 : kk * 32) >> 4), db + ((bmn ? kk * 2048 : kk * 32) >> 4),
-                                    idesc, (kc | kk) != 0);
+                        const uint64_t oa = (amn ? kk * 2048 : kk * 32) >> 4, ob = (bmn ? kk * 2048 : kk * 32) >> 4;
+                        if (kc * kDepth + kk * 16 < deep) {
+                            if constexpr (PAIR) mma_f16_pair(d_tmem, da + oa, db + ob, idesc, (kc | kk) != 0);
+                            else mma_f16(d_tmem, da + oa, db + ob, idesc, (kc | kk) != 0);
+                        }
                     }
-                    mma_commit(empty(stage));
+                    if constexpr (PAIR) mma_commit_pair(empty(stage));
+                    else mma_commit(empty(stage));
                     if (++stage == NS) { stage = 0; phase ^= 1u; }
                 }
                 if (!ok) break;
-                mma_commit(accf(abuf));
+                if constexpr (PAIR) mma_commit_pair(accf(abuf));
+                else mma_commit(accf(abuf));
                 abuf ^= 1u;
                 if (abuf == 0) aphase ^= 1u;
             }
             if (!ok) {                                     // a timeout: the MMAs issued so far end before TMEM is freed
-                mma_commit(drain);
+                if constexpr (PAIR) mma_commit_pair(drain);
+                else mma_commit(drain);
                 for (uint32_t n = 0; n < kSpinLimit && !mbar_try(drain, 0); n++) {}
             }
         }
@@ -343,14 +368,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                  i < a.pairs * a.ldo; i += (int64_t)gridDim.x * kEpiThreads)
                 out[i] = Elem<T>::from(0.0f);
         }
-        for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-            const Tile w = walk.at(a, first, t);
+        for (int64_t t = t0; t < tiles && ok; t += dt) {
+            const Tile w = Sh::at(a, first, t, e);
             if (w.steps > 0) {
                 ok = mbar_wait(accf(abuf), aphase, abort_flag);
                 if (!ok) break;
                 tc_fence_after();
             }
-            const int f = w.f0 + 32 * q + lane;
+            const int f = w.f0 + rank * kFeat + 32 * q + lane;
             for (int c = 0; c < w.ncols; c += 32) {
                 float v[32];
                 if (w.steps > 0) {
@@ -389,18 +414,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             if (w.steps > 0) {
                 tc_fence_before();
-                mbar_arrive(acce(abuf));
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (PAIR) mbar_arrive_cluster(cluster_addr(acce(abuf), 0));
+                    else mbar_arrive(acce(abuf));
+                }
                 abuf ^= 1u;
                 if (abuf == 0) aphase ^= 1u;
             }
         }
     }
 
+    __syncwarp();
     tc_fence_before();
-    __syncthreads();
+    if constexpr (PAIR) cluster_sync();
+    else __syncthreads();
     if (warp == 0) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * COLS));
+        if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * COLS));
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * COLS));
     }
     if (threadIdx.x == 0 && *abort_flag) atomicExch(a.error, 1);
 }
@@ -422,20 +454,31 @@ bool make_map(CUtensorMap* m, int dtype, const void* base, int64_t cols, int64_t
     return r == CUDA_SUCCESS;
 }
 
-template <typename T, int MODE, int COLS, bool GATHER>
+template <typename T, int MODE, int COLS, bool GATHER, bool PAIR>
 cudaError_t run_tc(const CUtensorMap (&m)[4], const TcArgs& a, cudaStream_t st) {
-    auto kern = k_expert_tc<T, MODE, COLS, GATHER>;
-    const size_t smem = TcSmem<COLS>::base + (size_t)(a.experts + 1) * 4;
+    auto kern = k_expert_tc<T, MODE, COLS, GATHER, PAIR>;
+    using S = TcSmem<COLS, PAIR>;
     static unsigned long long configured = 0;
     int dev = 0;
     cudaGetDevice(&dev);
     if (!(configured >> (dev & 63) & 1ull)) {
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             TcSmem<COLS>::base + TcSmem<COLS>::EXPERTS);
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::base + S::EXPERTS);
         if (e != cudaSuccess) return e;
         configured |= 1ull << (dev & 63);
     }
-    return launch_pdl(kern, dim3(num_sms()), dim3(kTcThreads), smem, st, m[0], m[1], m[2], m[3], a);
+    const size_t smem = S::base + (size_t)(a.experts + 1) * 4;
+    const int grid = PAIR ? num_sms() / 2 * 2 : num_sms();
+    if constexpr (PAIR) return launch_pdl_clusters(kern, dim3(grid), dim3(kTcThreads), smem, st, 2, m[0], m[1], m[2], m[3], a);
+    return launch_pdl(kern, dim3(grid), dim3(kTcThreads), smem, st, m[0], m[1], m[2], m[3], a);
+}
+
+// The pair's 256 features where there are more than 128; one CTA's 128 otherwise.
+template <typename T, int MODE, int COLS, bool GATHER>
+cudaError_t run_shape(const CUtensorMap (&m)[4], const TcArgs& a, cudaStream_t st) {
+    if constexpr (COLS == 256) {
+        if (a.feats > kFeat) return run_tc<T, MODE, COLS, GATHER, true>(m, a, st);
+    }
+    return run_tc<T, MODE, COLS, GATHER, false>(m, a, st);
 }
 
 template <typename T>
@@ -443,27 +486,26 @@ cudaError_t run_kind(const ExpertCall& c, const Operands& o, cudaStream_t st) {
     CUtensorMap m[4];
     TcArgs a = {};
     a.offsets = c.offsets;
-    a.rows = c.rows;
+    a.rows = o.rows;
+    a.x_rows = o.x_rows;
     a.pairs = (int)c.pairs;
     a.experts = c.experts;
     a.error = c.error;
+    const bool few = expert_few_rows(c);
     bool ok;
-    // positions per tile: 64 where the experts' mean is below that (a stage is then 24 KB and eight are in flight)
-    const bool few = c.pairs <= (int64_t)c.experts * 64;
     switch (c.kind) {
         case kExpertForward:
-            a.x_rows = c.x_rows;
             a.feats = c.n;
             a.depth = c.d;
             a.out = c.y;
             a.ldo = c.n;
             ok = make_map(&m[0], c.dtype, o.w, c.d, c.n, c.experts, o.ldw, kFeat) &&
-                 make_map(&m[2], c.dtype, o.x, c.d, c.x_rows, 0, o.ldx, 32) &&
-                 make_map(&m[3], c.dtype, o.x, c.d, c.x_rows, 0, o.ldx, 1);
+                 make_map(&m[2], c.dtype, o.x, c.d, o.x_rows, 0, o.ldx, 32) &&
+                 make_map(&m[3], c.dtype, o.x, c.d, o.x_rows, 0, o.ldx, 1);
             m[1] = m[0];
             if (!ok) return cudaErrorInvalidValue;
-            if (c.rows) return few ? run_tc<T, kExpertForward, 64, true>(m, a, st) : run_tc<T, kExpertForward, 256, true>(m, a, st);
-            return few ? run_tc<T, kExpertForward, 64, false>(m, a, st) : run_tc<T, kExpertForward, 256, false>(m, a, st);
+            if (few) return o.rows ? run_shape<T, kExpertForward, 64, true>(m, a, st) : run_shape<T, kExpertForward, 64, false>(m, a, st);
+            return run_shape<T, kExpertForward, 256, false>(m, a, st);
         case kExpertDx:
             a.rows = nullptr;
             a.x_rows = c.pairs;
@@ -476,9 +518,8 @@ cudaError_t run_kind(const ExpertCall& c, const Operands& o, cudaStream_t st) {
             m[1] = m[0];
             m[3] = m[2];
             if (!ok) return cudaErrorInvalidValue;
-            return few ? run_tc<T, kExpertDx, 64, false>(m, a, st) : run_tc<T, kExpertDx, 256, false>(m, a, st);
+            return few ? run_shape<T, kExpertDx, 64, false>(m, a, st) : run_shape<T, kExpertDx, 256, false>(m, a, st);
         default:
-            a.x_rows = c.x_rows;
             a.feats = c.n;
             a.cols = c.d;
             a.out = c.dw;
@@ -486,10 +527,10 @@ cudaError_t run_kind(const ExpertCall& c, const Operands& o, cudaStream_t st) {
             a.out_vec = c.d % 8 == 0 && reinterpret_cast<uintptr_t>(c.dw) % 16 == 0;
             ok = make_map(&m[0], c.dtype, o.dy, c.n, c.pairs, 0, o.lddy, kDepth) &&
                  make_map(&m[1], c.dtype, o.dy, c.n, c.pairs, 0, o.lddy, 1) &&
-                 make_map(&m[2], c.dtype, o.x, c.d, c.x_rows, 0, o.ldx, kDepth) &&
-                 make_map(&m[3], c.dtype, o.x, c.d, c.x_rows, 0, o.ldx, 1);
+                 make_map(&m[2], c.dtype, o.x, c.d, o.x_rows, 0, o.ldx, kDepth) &&
+                 make_map(&m[3], c.dtype, o.x, c.d, o.x_rows, 0, o.ldx, 1);
             if (!ok) return cudaErrorInvalidValue;
-            return c.rows ? run_tc<T, kExpertDw, 256, true>(m, a, st) : run_tc<T, kExpertDw, 256, false>(m, a, st);
+            return run_shape<T, kExpertDw, 256, false>(m, a, st);
     }
 }
 

@@ -1,8 +1,13 @@
-// experts.cu -- products per expert: which kernel a call takes, and the copies of operands that TMA cannot read.
+// experts.cu -- products per expert: which kernel a call takes, and the copies of operands that TMA cannot read fast.
 //
 // TMA wants a base on 16 bytes and rows a multiple of 16 bytes apart.  An operand that is not so (an odd number of
 // columns, a view that starts anywhere) is first copied to the workspace with its rows padded to 8 elements; the
 // padding is never read as data (the tensor maps end at the true column).
+//
+// Rows of x read by index: with few rows an expert the products' kernel gathers them itself (tile::gather4).  A gather
+// of four 128-byte pieces took 36 cycles of the TMA unit however it was issued, so a tile of 256 positions spent four
+// times as long on them as on its MMAs (8192 x 8 of 64 experts, 2048 x 2048: 2365 us, from grouped rows 529 us); with
+// many rows an expert, and for dW, they are copied in grouped order first.
 #include "common.cuh"
 #include "experts.cuh"
 #include "kmc_internal.h"
@@ -11,32 +16,48 @@ namespace kmc {
 
 namespace {
 
-constexpr int kPadThreads = 256;
+constexpr int kTakeThreads = 256;
 
 bool readable(const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; }
 int64_t padded(int64_t cols) { return (cols + 7) / 8 * 8; }
 size_t a256(size_t v) { return (v + 255) & ~size_t(255); }
+bool takes_x(const ExpertCall& c) { return c.x && c.rows && !(c.kind == kExpertForward && expert_few_rows(c)); }
 
-// rows x cols elements, ld apart, to rows ldp apart: a thread writes 16 bytes
-__global__ void __launch_bounds__(kPadThreads)
-    k_pad_rows(const uint16_t* __restrict__ src, int64_t rows, int cols, int64_t ld, int ldp, uint16_t* __restrict__ dst) {
+// dst row i (cols elements, ldp apart) = src row idx[i], or row i without idx; zeros for a row outside src and in the
+// padding.  A thread writes 16 bytes; it reads them as one (VEC) or element by element.
+template <bool VEC>
+__global__ void __launch_bounds__(kTakeThreads)
+    k_take(const uint16_t* __restrict__ src, int64_t src_rows, const int32_t* __restrict__ idx, int64_t rows, int cols,
+           int64_t ld, int ldp, uint16_t* __restrict__ dst) {
     pdl_wait();
     const int vecs = ldp / 8;
-    const int64_t i = (int64_t)blockIdx.x * kPadThreads + threadIdx.x;
+    const int64_t i = (int64_t)blockIdx.x * kTakeThreads + threadIdx.x;
     if (i >= rows * vecs) return;
     const int64_t r = i / vecs;
     const int c = (int)(i - r * vecs) * 8;
-    Pack<uint16_t, 8> p;
+    const int64_t s = idx ? (int64_t)__ldg(idx + r) : r;
+    Pack<uint16_t, 8> p = {};
+    if (s >= 0 && s < src_rows) {
+        if constexpr (VEC) {
+            p = *reinterpret_cast<const Pack<uint16_t, 8>*>(src + s * ld + c);
+        } else {
 #pragma unroll
-    for (int j = 0; j < 8; j++) p.v[j] = c + j < cols ? src[r * ld + c + j] : (uint16_t)0;
+            for (int j = 0; j < 8; j++)
+                if (c + j < cols) p.v[j] = src[s * ld + c + j];
+        }
+    }
     *reinterpret_cast<Pack<uint16_t, 8>*>(dst + r * ldp + c) = p;
 }
 
-cudaError_t pad(const void** p, int64_t* ld, int64_t rows, int cols, char** ws, cudaStream_t st) {
-    if (readable(*p, *ld)) return cudaSuccess;
-    const int64_t ldp = padded(cols), blocks = (rows * (ldp / 8) + kPadThreads - 1) / kPadThreads;
-    cudaError_t e = launch_pdl(k_pad_rows, dim3((unsigned)blocks), dim3(kPadThreads), 0, st,
-                               static_cast<const uint16_t*>(*p), rows, cols, *ld, (int)ldp, reinterpret_cast<uint16_t*>(*ws));
+// Replaces the operand at *p by its copy in the workspace
+cudaError_t take(const void** p, int64_t* ld, int64_t src_rows, const int32_t* idx, int64_t rows, int cols, char** ws,
+                 cudaStream_t st) {
+    const int64_t ldp = padded(cols), blocks = (rows * (ldp / 8) + kTakeThreads - 1) / kTakeThreads;
+    if (blocks >= INT32_MAX) return cudaErrorInvalidValue;
+    const bool vec = readable(*p, *ld) && cols % 8 == 0;
+    cudaError_t e = launch_pdl(vec ? k_take<true> : k_take<false>, dim3((unsigned)blocks), dim3(kTakeThreads), 0, st,
+                               static_cast<const uint16_t*>(*p), src_rows, idx, rows, cols, *ld, (int)ldp,
+                               reinterpret_cast<uint16_t*>(*ws));
     *p = *ws;
     *ld = ldp;
     *ws += a256((size_t)rows * ldp * 2);
@@ -45,9 +66,14 @@ cudaError_t pad(const void** p, int64_t* ld, int64_t rows, int cols, char** ws, 
 
 }  // namespace
 
+// Positions per tile: 64 where the experts' mean is at most that (a stage is then 24 KB and eight are in flight), 256
+// above.
+bool expert_few_rows(const ExpertCall& c) { return c.pairs <= (int64_t)c.experts * 64; }
+
 size_t expert_bytes(const ExpertCall& c) {
     size_t need = 0;
-    if (c.x && !readable(c.x, c.ldx)) need += a256((size_t)c.x_rows * padded(c.d) * 2);
+    if (takes_x(c)) need += a256((size_t)c.pairs * padded(c.d) * 2);
+    else if (c.x && !readable(c.x, c.ldx)) need += a256((size_t)c.x_rows * padded(c.d) * 2);
     if (c.w && !readable(c.w, c.d)) need += a256((size_t)c.experts * c.n * padded(c.d) * 2);
     if (c.dy && !readable(c.dy, c.n)) need += a256((size_t)c.pairs * padded(c.n) * 2);
     return need;
@@ -58,12 +84,21 @@ cudaError_t launch_expert(const ExpertCall& c, cudaStream_t st) {
         return c.kind == kExpertForward ? cudaMemsetAsync(c.y, 0, (size_t)c.pairs * c.n * 2, st)
                                         : cudaMemsetAsync(c.dw, 0, (size_t)c.experts * c.n * c.d * 2, st);
     if (c.pairs == 0) return cudaMemsetAsync(c.dw, 0, (size_t)c.experts * c.n * c.d * 2, st);
-    Operands o = {c.x, c.w, c.dy, c.ldx, c.d, c.n};
+    Operands o = {c.x, c.w, c.dy, c.ldx, c.d, c.n, c.rows, c.x_rows};
     char* ws = static_cast<char*>(c.ws);
     cudaError_t e = cudaSuccess;
-    if (o.x) e = pad(&o.x, &o.ldx, c.x_rows, c.d, &ws, st);
-    if (e == cudaSuccess && o.w) e = pad(&o.w, &o.ldw, (int64_t)c.experts * c.n, c.d, &ws, st);
-    if (e == cudaSuccess && o.dy) e = pad(&o.dy, &o.lddy, c.pairs, c.n, &ws, st);
+    if (takes_x(c)) {
+        e = take(&o.x, &o.ldx, c.x_rows, c.rows, c.pairs, c.d, &ws, st);
+        o.rows = nullptr;
+        o.x_rows = c.pairs;
+    } else if (o.x && !readable(o.x, o.ldx)) {
+        e = take(&o.x, &o.ldx, c.x_rows, nullptr, c.x_rows, c.d, &ws, st);
+    }
+    if (e == cudaSuccess && o.w && !readable(o.w, o.ldw)) {
+        const int64_t rows = (int64_t)c.experts * c.n;
+        e = take(&o.w, &o.ldw, rows, nullptr, rows, c.d, &ws, st);
+    }
+    if (e == cudaSuccess && o.dy && !readable(o.dy, o.lddy)) e = take(&o.dy, &o.lddy, c.pairs, nullptr, c.pairs, c.n, &ws, st);
     return e == cudaSuccess ? launch_expert_tc(c, o, st) : e;
 }
 

@@ -27,6 +27,27 @@ cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t sme
     return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
 }
 
+// The same in clusters of `ctas` consecutive CTAs.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_pdl_clusters(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, int ctas,
+                                Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = ctas;
+    at[1].val.clusterDim.y = 1;
+    at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
+
 // Arguments of the pass kernels.
 struct PassArgs {
     const float* X;
@@ -267,13 +288,16 @@ struct ExpertCall {
     void* ws;                 // expert_bytes(call) bytes
     int* error;               // set to 1 by a kernel that gave up on a barrier
 };
-size_t expert_bytes(const ExpertCall& c);   // by the operands' pointers, sizes and row strides
+size_t expert_bytes(const ExpertCall& c);   // by the call's kind, operands, sizes and row strides
 cudaError_t launch_expert(const ExpertCall& c, cudaStream_t st);
 // the 16-bit operands as the tensor-core kernel reads them: 16-byte aligned, rows a multiple of 8 elements apart
 struct Operands {
     const void *x, *w, *dy;
     int64_t ldx, ldw, lddy;
+    const int32_t* rows;      // row of x per position; nullptr: grouped already
+    int64_t x_rows;
 };
+bool expert_few_rows(const ExpertCall& c);
 cudaError_t launch_expert_tc(const ExpertCall& c, const Operands& o, cudaStream_t st);
 
 }  // namespace kmc

@@ -232,24 +232,21 @@ def _check_expert(x, w, groups, gather):
     return T, k
 
 
-def _workspace(x, w, dy, P, E, N, D, device):
-    """Room for padded copies of operands that do not start, or continue from row to row, on 16-byte boundaries."""
-    ldx = max(x.stride(0), D) if x is not None else D
-    at = (0 if x is None else x.data_ptr() | ldx * 2) | (0 if w is None else w.data_ptr() | D * 2)
-    at |= 0 if dy is None else dy.data_ptr() | N * 2
-    if at % 16 == 0:
-        return None, 0
-    nb = int(_lib.load().kmc_expert_bytes(_ptr(x), 0 if x is None else x.shape[0], ldx, _ptr(w), _ptr(dy), P, E, N, D))
+def _workspace(x, rows, w, dy, P, E, N, D, device):
+    """The workspace of an expert product: for x in grouped order, and for padded copies of unaligned operands."""
+    x_rows, ldx = (x.shape[0], max(x.stride(0), D)) if x is not None else (0, D)
+    nb = _lib.load().kmc_expert_bytes(_ptr(x), x_rows, ldx, _ptr(rows), _ptr(w), _ptr(dy), P, E, N, D)
     return (torch.empty(nb, dtype=torch.uint8, device=device) if nb else None), nb
 
 
 def _expert(x, w, groups, gather):
     (E, N, D), P, dev = w.shape, groups.rows.numel(), w.device
     y = torch.empty((P, N), dtype=w.dtype, device=dev)
-    ws, nb = _workspace(x, w, None, P, E, N, D, dev)
+    rows = groups.rows if gather else None
+    ws, nb = _workspace(x, rows, w, None, P, E, N, D, dev)
     with _on(dev):
         _lib.call("kmc_expert_matmul", x.data_ptr(), x.shape[0], max(x.stride(0), D),
-                  groups.rows.data_ptr() if gather else None, w.data_ptr(), groups.offsets.data_ptr(), P, E, N, D,
+                  _ptr(rows), w.data_ptr(), groups.offsets.data_ptr(), P, E, N, D,
                   _DTYPES[w.dtype], y.data_ptr(), _ptr(ws), nb, _error_word(dev).data_ptr(), _stream())
     return y
 
@@ -257,7 +254,7 @@ def _expert(x, w, groups, gather):
 def _expert_dx(dy, w, groups, gather):
     (E, N, D), P, dev = w.shape, groups.rows.numel(), w.device
     dx = torch.empty((P, D), dtype=w.dtype, device=dev)
-    ws, nb = _workspace(None, w, dy, P, E, N, D, dev)
+    ws, nb = _workspace(None, None, w, dy, P, E, N, D, dev)
     with _on(dev):
         _lib.call("kmc_expert_matmul_dx", dy.data_ptr(), w.data_ptr(), groups.offsets.data_ptr(), P, E, N, D,
                   _DTYPES[w.dtype], dx.data_ptr(), _ptr(ws), nb, _error_word(dev).data_ptr(), _stream())
@@ -269,10 +266,11 @@ def _expert_dx(dy, w, groups, gather):
 def _expert_dw(dy, x, groups, E, gather):
     (N, D), P, dev = (dy.shape[1], x.shape[1]), groups.rows.numel(), dy.device
     dw = torch.empty((E, N, D), dtype=x.dtype, device=dev)
-    ws, nb = _workspace(x, None, dy, P, E, N, D, dev)
+    rows = groups.rows if gather else None
+    ws, nb = _workspace(x, rows, None, dy, P, E, N, D, dev)
     with _on(dev):
         _lib.call("kmc_expert_matmul_dw", dy.data_ptr(), x.data_ptr(), x.shape[0], max(x.stride(0), D),
-                  groups.rows.data_ptr() if gather else None, groups.offsets.data_ptr(), P, E, N, D,
+                  _ptr(rows), groups.offsets.data_ptr(), P, E, N, D,
                   _DTYPES[x.dtype], dw.data_ptr(), _ptr(ws), nb, _error_word(dev).data_ptr(), _stream())
     return dw
 
