@@ -38,8 +38,10 @@ namespace {
 constexpr int kFeat = 128;                // features per CTA and tile (the MMA's M, or half of it)
 constexpr int kDepth = 64;                // depth per stage: one 128-byte swizzle row of 16-bit elements
 constexpr int kBox = 64 * kDepth * 2;     // 64 x 64 elements
+constexpr int kBlock = 8;                 // position tiles per block of the tile order
 constexpr int kTcThreads = 192;
 constexpr int kEpiThreads = 128;
+constexpr int kEpiBytes = 32 * 80;        // a warp's 32 x 32 results on their way from TMEM to memory
 constexpr unsigned kFull = 0xffffffffu;
 
 struct TcArgs {
@@ -52,7 +54,7 @@ struct TcArgs {
     int depth;                            // forward: d, dx: n; dW: per expert
     void* out;
     int64_t ldo;                          // row length of out
-    int out_vec;                          // dW: rows of out start on 16-byte boundaries
+    int out_vec;                          // rows of out start on 16-byte boundaries
     int* error;
 };
 
@@ -63,10 +65,11 @@ struct TcSmem {
     static constexpr int B = MINE * kDepth * 2;
     static constexpr int STAGE = A + B;
     static constexpr int BAR = 256;
+    static constexpr int EPI = 4 * kEpiBytes;
     static constexpr int EXPERTS = (kGroupMaxExperts + 1) * 4;
-    static constexpr int FREE = 227 * 1024 - BAR - EXPERTS - 2048;   // 1 KB to align, 1 KB of static arrays
+    static constexpr int FREE = 227 * 1024 - BAR - EPI - EXPERTS - 2048;   // 1 KB to align, 1 KB of static arrays
     static constexpr int NS = FREE / STAGE > 8 ? 8 : FREE / STAGE;
-    static constexpr int base = NS * STAGE + BAR + 1024;      // + the experts' tile counts
+    static constexpr int base = NS * STAGE + BAR + EPI + 1024;      // + the experts' tile counts
     static_assert(NS >= 2 && 8 * (2 * NS + 5) + 8 <= BAR, "barrier block");
 };
 
@@ -103,17 +106,22 @@ struct Shape {
         const int size = rows(count);
         return (count + size - 1) / size;
     }
-    // Tile t; `e` walks up with t, first[e] = tiles of the experts before e.
+    // Tile t; `e` walks up with t, first[e] = tiles of the experts before e.  An expert's tiles go in blocks of kBlock
+    // position tiles (dW: column tiles) by all feature tiles, positions fastest, so the tiles that run at the same time
+    // read about as many rows of the one operand as of the other, and the L2 serves them.
     static __device__ __forceinline__ Tile at(const TcArgs& a, const int* first, int64_t t, int& e) {
         Tile r;
         const int ft = feature_tiles(a), j = (int)(t / ft);
-        r.f0 = (int)(t - (int64_t)j * ft) * FEATS;
         while (j >= first[e + 1]) e++;
+        const int in = (int)(t - (int64_t)first[e] * ft), block = in / (kBlock * ft);
+        const int left = first[e + 1] - first[e] - block * kBlock, wide = left < kBlock ? left : kBlock;
+        const int k = in - block * kBlock * ft, tile = block * kBlock + k % wide;
+        r.f0 = k / wide * FEATS;
         r.e = e;
         int begin, count;
         segment(a, e, begin, count);
         if constexpr (MODE == kExpertDw) {
-            r.c0 = (j - first[e]) * COLS;
+            r.c0 = tile * COLS;
             r.p0 = begin;
             r.p1 = begin + count;
             r.ncols = min((a.cols - r.c0 + STEP - 1) / STEP * STEP, COLS);
@@ -121,7 +129,7 @@ struct Shape {
         } else {
             const int size = rows(count);
             r.c0 = 0;
-            r.p0 = begin + (j - first[e]) * size;
+            r.p0 = begin + tile * size;
             r.p1 = min(r.p0 + size, begin + count);
             r.ncols = (r.p1 - r.p0 + STEP - 1) / STEP * STEP;
             r.steps = (a.depth + kDepth - 1) / kDepth;
@@ -153,6 +161,80 @@ __device__ __forceinline__ void gather4(uint32_t dst, const CUtensorMap* m, int 
     else tma_gather4(dst, m, x, r, bar);
 }
 
+// Stores a warp's 32 features (lanes) x 32 columns of the accumulator.  A lane's values are 2 bytes of 32 different
+// rows of out (positions) or 64 bytes of one (dW): written as they are, a tile of 256 columns took 19650 cycles, more
+// than its MMAs up to a depth of 2500.  So they go through shared memory and leave as 16-byte pieces of 64-byte runs.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    Pack<T, 2> p;
+    p.v[0] = Elem<T>::from(lo);
+    p.v[1] = Elem<T>::from(hi);
+    return *reinterpret_cast<const uint32_t*>(&p);
+}
+
+// Column j is row j of dst (ldo apart), the lanes its 32 consecutive features; rows below `left`, features below
+// `feats` exist.
+template <typename T>
+__device__ __forceinline__ void store_positions(T* dst, int64_t ldo, int left, int feats, bool vec, const float (&v)[32],
+                                                unsigned char* stash) {
+    const int lane = threadIdx.x & 31;
+    if (vec) {
+        // word [j / 2][lane] = columns j and j + 1 of the lane's feature; a lane then takes the words of 8 features
+        // and separates them into 16 bytes of row j and 16 of row j + 1
+        uint32_t* w = reinterpret_cast<uint32_t*>(stash);
+#pragma unroll
+        for (int j = 0; j < 16; j++) w[j * 36 + lane] = pack2<T>(v[2 * j], v[2 * j + 1]);
+        __syncwarp();
+        const int g = (lane & 3) * 8;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int j = (lane >> 2) + 8 * i;
+            const uint4 a = *reinterpret_cast<const uint4*>(w + j * 36 + g), b = *reinterpret_cast<const uint4*>(w + j * 36 + g + 4);
+            const uint4 lo = make_uint4(__byte_perm(a.x, a.y, 0x5410), __byte_perm(a.z, a.w, 0x5410),
+                                        __byte_perm(b.x, b.y, 0x5410), __byte_perm(b.z, b.w, 0x5410));
+            const uint4 hi = make_uint4(__byte_perm(a.x, a.y, 0x7632), __byte_perm(a.z, a.w, 0x7632),
+                                        __byte_perm(b.x, b.y, 0x7632), __byte_perm(b.z, b.w, 0x7632));
+            if (g < feats) {                               // feats is a multiple of 8 here
+                T* to = dst + (int64_t)(2 * j) * ldo + g;
+                if (2 * j < left) *reinterpret_cast<uint4*>(to) = lo;
+                if (2 * j + 1 < left) *reinterpret_cast<uint4*>(to + ldo) = hi;
+            }
+        }
+        __syncwarp();
+    } else if (lane < feats) {
+#pragma unroll
+        for (int j = 0; j < 32; j++)
+            if (j < left) dst[(int64_t)j * ldo + lane] = Elem<T>::from(v[j]);
+    }
+}
+
+// The lanes are 32 rows of dst (ldo apart), the columns its consecutive elements; `left` columns and `feats` rows exist.
+template <typename T>
+__device__ __forceinline__ void store_features(T* dst, int64_t ldo, int left, int feats, bool vec, const float (&v)[32],
+                                               unsigned char* stash) {
+    const int lane = threadIdx.x & 31;
+    if (vec) {
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+            *reinterpret_cast<uint4*>(stash + lane * 80 + g * 16) =
+                make_uint4(pack2<T>(v[8 * g], v[8 * g + 1]), pack2<T>(v[8 * g + 2], v[8 * g + 3]),
+                           pack2<T>(v[8 * g + 4], v[8 * g + 5]), pack2<T>(v[8 * g + 6], v[8 * g + 7]));
+        __syncwarp();
+        const int g = lane & 3;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = (lane >> 2) + 8 * i;
+            if (r < feats && g * 8 < left)                 // left is a multiple of 8 here
+                *reinterpret_cast<uint4*>(dst + r * ldo + g * 8) = *reinterpret_cast<const uint4*>(stash + r * 80 + g * 16);
+        }
+        __syncwarp();
+    } else if (lane < feats) {
+#pragma unroll
+        for (int j = 0; j < 32; j++)
+            if (j < left) dst[lane * ldo + j] = Elem<T>::from(v[j]);
+    }
+}
+
 template <typename T, int MODE, int COLS, bool GATHER, bool PAIR>
 __global__ void __launch_bounds__(kTcThreads, 1)
     k_expert_tc(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap ma_row,
@@ -174,7 +256,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t drain = bars + 8u * (2 * NS + 4);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbars + 8 * (2 * NS + 5));
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gbars + 8 * (2 * NS + 5) + 4);
-    int* first = reinterpret_cast<int*>(gbars + S::BAR);
+    unsigned char* stash = gbars + S::BAR;
+    int* first = reinterpret_cast<int*>(gbars + S::BAR + S::EPI);
     __shared__ int part[kTcThreads / 32];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -241,8 +324,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         uint32_t phase = 0;
         int64_t issued = 0;
         bool ok = true;
+        Tile next;
+        if (t0 < tiles) next = Sh::at(a, first, t0, e);
         for (int64_t t = t0; t < tiles && ok; t += dt) {
-            const Tile w = Sh::at(a, first, t, e);
+            const Tile w = next;
+            if (w.steps == 0) {
+                if (t + dt < tiles) next = Sh::at(a, first, t + dt, e);
+                continue;
+            }
             const int f0 = w.f0 + rank * kFeat;
             const int half = w.ncols / CTAS;               // columns of this CTA's operand
             int r[4];                                      // rows of this lane's gather
@@ -294,6 +383,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                 }
                 issued++;
+                if (kc == 0 && t + dt < tiles) next = Sh::at(a, first, t + dt, e);
                 if (++stage == NS) { stage = 0; phase ^= 1u; }
             }
         }
@@ -315,9 +405,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             int stage = 0;
             uint32_t phase = 0, abuf = 0, aphase = 0;
             bool ok = true;
+            // the next tile is worked out while this one's MMAs run: about 1000 cycles (two loads, three divisions)
+            // that would otherwise pass between the last MMA of a tile and the first of the next
+            Tile next;
+            if (t0 < tiles) next = Sh::at(a, first, t0, e);
             for (int64_t t = t0; t < tiles && ok; t += dt) {
-                const Tile w = Sh::at(a, first, t, e);
-                if (w.steps == 0) continue;                // dW of an expert with no rows: nothing to add up
+                const Tile w = next;
+                if (w.steps == 0) {                        // dW of an expert with no rows: nothing to add up
+                    if (t + dt < tiles) next = Sh::at(a, first, t + dt, e);
+                    continue;
+                }
                 ok = mbar_wait(acce(abuf), aphase ^ 1u, abort_flag);
                 if (!ok) break;
                 tc_fence_after();
@@ -341,6 +438,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                     if constexpr (PAIR) mma_commit_pair(empty(stage));
                     else mma_commit(empty(stage));
+                    if (kc == 0 && t + dt < tiles) next = Sh::at(a, first, t + dt, e);
                     if (++stage == NS) { stage = 0; phase ^= 1u; }
                 }
                 if (!ok) break;
@@ -360,6 +458,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int q = warp & 3;
         const uint32_t lane_base = tmem + ((uint32_t)(32 * q) << 16);
         T* out = static_cast<T*>(a.out);
+        unsigned char* mine = stash + q * kEpiBytes;
         uint32_t abuf = 0, aphase = 0;
         bool ok = true;
         if constexpr (MODE != kExpertDw) {                 // rows past the last group: zeros
@@ -375,8 +474,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (!ok) break;
                 tc_fence_after();
             }
-            const int f = w.f0 + rank * kFeat + 32 * q + lane;
-            for (int c = 0; c < w.ncols; c += 32) {
+            const int f = w.f0 + rank * kFeat + 32 * q;    // the warp's first feature
+            for (int c = 0; c < w.ncols && f < a.feats; c += 32) {
                 float v[32];
                 if (w.steps > 0) {
                     tmem_ld32(lane_base + abuf * COLS + c, v);
@@ -384,33 +483,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
                     for (int j = 0; j < 32; j++) v[j] = 0.0f;
                 }
-                if constexpr (MODE == kExpertDw) {
-                    if (f < a.feats) {
-                        T* dst = out + ((int64_t)w.e * a.feats + f) * a.ldo + w.c0 + c;
-                        const int left = a.cols - w.c0 - c;
-#pragma unroll
-                        for (int g = 0; g < 4; g++) {
-                            if (a.out_vec && g * 8 + 8 <= left) {
-                                Pack<T, 8> p;
-#pragma unroll
-                                for (int j = 0; j < 8; j++) p.v[j] = Elem<T>::from(v[g * 8 + j]);
-                                *reinterpret_cast<Pack<T, 8>*>(dst + g * 8) = p;
-                            } else {
-#pragma unroll
-                                for (int j = 0; j < 8; j++)
-                                    if (g * 8 + j < left) dst[g * 8 + j] = Elem<T>::from(v[g * 8 + j]);
-                            }
-                        }
-                    }
-                } else {
-                    if (f < a.feats) {
-                        const int left = w.p1 - w.p0 - c;
-                        T* dst = out + (int64_t)(w.p0 + c) * a.ldo + f;
-#pragma unroll
-                        for (int j = 0; j < 32; j++)
-                            if (j < left) dst[j * a.ldo] = Elem<T>::from(v[j]);
-                    }
-                }
+                if constexpr (MODE == kExpertDw)
+                    store_features<T>(out + ((int64_t)w.e * a.feats + f) * a.ldo + w.c0 + c, a.ldo, a.cols - w.c0 - c,
+                                      a.feats - f, a.out_vec, v, mine);
+                else
+                    store_positions<T>(out + (int64_t)(w.p0 + c) * a.ldo + f, a.ldo, w.p1 - w.p0 - c, a.feats - f, a.out_vec,
+                                       v, mine);
             }
             if (w.steps > 0) {
                 tc_fence_before();
@@ -492,12 +570,14 @@ cudaError_t run_kind(const ExpertCall& c, const Operands& o, cudaStream_t st) {
     a.experts = c.experts;
     a.error = c.error;
     const bool few = expert_few_rows(c);
+    auto whole = [](const void* p, int cols) { return cols % 8 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0; };
     bool ok;
     switch (c.kind) {
         case kExpertForward:
             a.feats = c.n;
             a.depth = c.d;
             a.out = c.y;
+            a.out_vec = whole(c.y, c.n);
             a.ldo = c.n;
             ok = make_map(&m[0], c.dtype, o.w, c.d, c.n, c.experts, o.ldw, kFeat) &&
                  make_map(&m[2], c.dtype, o.x, c.d, o.x_rows, 0, o.ldx, 32) &&
@@ -512,6 +592,7 @@ cudaError_t run_kind(const ExpertCall& c, const Operands& o, cudaStream_t st) {
             a.feats = c.d;
             a.depth = c.n;
             a.out = c.dx;
+            a.out_vec = whole(c.dx, c.d);
             a.ldo = c.d;
             ok = make_map(&m[0], c.dtype, o.w, c.d, c.n, c.experts, o.ldw, kDepth) &&
                  make_map(&m[2], c.dtype, o.dy, c.n, c.pairs, 0, o.lddy, 32);
@@ -523,8 +604,8 @@ cudaError_t run_kind(const ExpertCall& c, const Operands& o, cudaStream_t st) {
             a.feats = c.n;
             a.cols = c.d;
             a.out = c.dw;
+            a.out_vec = whole(c.dw, c.d);
             a.ldo = c.d;
-            a.out_vec = c.d % 8 == 0 && reinterpret_cast<uintptr_t>(c.dw) % 16 == 0;
             ok = make_map(&m[0], c.dtype, o.dy, c.n, c.pairs, 0, o.lddy, kDepth) &&
                  make_map(&m[1], c.dtype, o.dy, c.n, c.pairs, 0, o.lddy, 1) &&
                  make_map(&m[2], c.dtype, o.x, c.d, o.x_rows, 0, o.ldx, kDepth) &&
