@@ -18,10 +18,13 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .core import _ptr, _stream
+from .core import _ptr
 
 _DTYPES = {torch.float32: _lib.KMC_F32, torch.bfloat16: _lib.KMC_BF16, torch.float16: _lib.KMC_F16}
 _SCORES = {"softmax": 0, "sigmoid": _lib.KMC_ROUTE_SIGMOID}
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+_fns = {}                           # entry points of libkmc.so, looked up once
 _errors = {}                        # per device: the int32 a kernel sets when it gave up on a barrier
 
 
@@ -49,20 +52,18 @@ def _check(t, name, ndim=None, dtypes=None, device=None):
     return t
 
 
-def _on(device):
-    """The tensors' device made current for a call (a no-op object when it already is)."""
-    return _NO_SWITCH if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-
-class _NoSwitch:
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        return False
-
-
-_NO_SWITCH = _NoSwitch()
+def _run(name, device, *args):
+    """kmc_<name>(*args, stream) on the device's current stream, the device made current for the call if it is not."""
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(_lib.load(), name)
+    if device.index == torch.cuda.current_device():
+        status = fn(*args, _raw_stream(device.index))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, _raw_stream(device.index))
+    if status:
+        _lib.check(status, name)
 
 
 def _rows_of(t):
@@ -75,7 +76,7 @@ def _error_word(device):
     if e is None:
         e = _errors[device] = torch.zeros(1, dtype=torch.int32, device=device)
         torch.cuda.current_stream(device).synchronize()      # zero before any stream's kernel can set it
-    return e
+    return e.data_ptr()
 
 
 def expert_status(device=None):
@@ -100,18 +101,16 @@ def _route(logits, top_k, flags, bias, groups, top_groups, scale, mask):
     T, E = logits.shape
     ids = torch.empty((T, top_k), dtype=torch.int32, device=logits.device)
     weights = torch.empty((T, top_k), dtype=torch.float32, device=logits.device)
-    with _on(logits.device):
-        _lib.call("kmc_route", logits.data_ptr(), _DTYPES[logits.dtype], T, E, max(logits.stride(0), E), _ptr(bias),
-                  _ptr(mask), top_k, groups, top_groups, scale, flags, ids.data_ptr(), weights.data_ptr(), _stream())
+    _run("kmc_route", logits.device, logits.data_ptr(), _DTYPES[logits.dtype], T, E, max(logits.stride(0), E), _ptr(bias),
+         _ptr(mask), top_k, groups, top_groups, scale, flags, ids.data_ptr(), weights.data_ptr())
     return ids, weights
 
 
 def _route_grad(dweights, logits, ids, flags, scale):
     T, E = logits.shape
     dlogits = torch.empty((T, E), dtype=logits.dtype, device=logits.device)
-    with _on(logits.device):
-        _lib.call("kmc_route_grad", dweights.data_ptr(), logits.data_ptr(), _DTYPES[logits.dtype], T, E,
-                  max(logits.stride(0), E), ids.data_ptr(), ids.shape[1], scale, flags, dlogits.data_ptr(), _stream())
+    _run("kmc_route_grad", logits.device, dweights.data_ptr(), logits.data_ptr(), _DTYPES[logits.dtype], T, E,
+         max(logits.stride(0), E), ids.data_ptr(), ids.shape[1], scale, flags, dlogits.data_ptr())
     return dlogits
 
 
@@ -194,9 +193,8 @@ def group_rows(ids, n_experts):
     offsets = torch.empty(max(E, 0) + 1, dtype=torch.int32, device=dev)
     rows = torch.empty(T * k, dtype=torch.int32, device=dev)
     slot = torch.empty(ids.shape, dtype=torch.int32, device=dev)
-    with _on(dev):
-        _lib.call("kmc_group_rows", ids.data_ptr(), T, k, E, offsets.data_ptr(), rows.data_ptr(), slot.data_ptr(),
-                  _ptr(ws), nb, _stream())
+    _run("kmc_group_rows", dev, ids.data_ptr(), T, k, E, offsets.data_ptr(), rows.data_ptr(), slot.data_ptr(),
+         _ptr(ws), nb)
     return RowGroups(offsets, rows, slot)
 
 
@@ -244,10 +242,9 @@ def _expert(x, w, groups, gather):
     y = torch.empty((P, N), dtype=w.dtype, device=dev)
     rows = groups.rows if gather else None
     ws, nb = _workspace(x, rows, w, None, P, E, N, D, dev)
-    with _on(dev):
-        _lib.call("kmc_expert_matmul", x.data_ptr(), x.shape[0], max(x.stride(0), D),
-                  _ptr(rows), w.data_ptr(), groups.offsets.data_ptr(), P, E, N, D,
-                  _DTYPES[w.dtype], y.data_ptr(), _ptr(ws), nb, _error_word(dev).data_ptr(), _stream())
+    _run("kmc_expert_matmul", dev, x.data_ptr(), x.shape[0], max(x.stride(0), D),
+         _ptr(rows), w.data_ptr(), groups.offsets.data_ptr(), P, E, N, D,
+         _DTYPES[w.dtype], y.data_ptr(), _ptr(ws), nb, _error_word(dev))
     return y
 
 
@@ -255,9 +252,8 @@ def _expert_dx(dy, w, groups, gather):
     (E, N, D), P, dev = w.shape, groups.rows.numel(), w.device
     dx = torch.empty((P, D), dtype=w.dtype, device=dev)
     ws, nb = _workspace(None, None, w, dy, P, E, N, D, dev)
-    with _on(dev):
-        _lib.call("kmc_expert_matmul_dx", dy.data_ptr(), w.data_ptr(), groups.offsets.data_ptr(), P, E, N, D,
-                  _DTYPES[w.dtype], dx.data_ptr(), _ptr(ws), nb, _error_word(dev).data_ptr(), _stream())
+    _run("kmc_expert_matmul_dx", dev, dy.data_ptr(), w.data_ptr(), groups.offsets.data_ptr(), P, E, N, D,
+         _DTYPES[w.dtype], dx.data_ptr(), _ptr(ws), nb, _error_word(dev))
     # a row with several choices: the float32 sum of its positions' gradients, which are in w's type by now (each
     # rounded once; the error of the sum stays within that of one more rounding of its result)
     return _combine(dx, groups, None) if gather else dx
@@ -268,10 +264,9 @@ def _expert_dw(dy, x, groups, E, gather):
     dw = torch.empty((E, N, D), dtype=x.dtype, device=dev)
     rows = groups.rows if gather else None
     ws, nb = _workspace(x, rows, None, dy, P, E, N, D, dev)
-    with _on(dev):
-        _lib.call("kmc_expert_matmul_dw", dy.data_ptr(), x.data_ptr(), x.shape[0], max(x.stride(0), D),
-                  _ptr(rows), groups.offsets.data_ptr(), P, E, N, D,
-                  _DTYPES[x.dtype], dw.data_ptr(), _ptr(ws), nb, _error_word(dev).data_ptr(), _stream())
+    _run("kmc_expert_matmul_dw", dev, dy.data_ptr(), x.data_ptr(), x.shape[0], max(x.stride(0), D),
+         _ptr(rows), groups.offsets.data_ptr(), P, E, N, D,
+         _DTYPES[x.dtype], dw.data_ptr(), _ptr(ws), nb, _error_word(dev))
     return dw
 
 
@@ -332,9 +327,8 @@ def _combine(y, groups, weights):
     slot = groups.slot
     T, k = slot.shape[0], (slot.shape[1] if slot.ndim == 2 else 1)
     out = torch.empty((T, y.shape[1]), dtype=y.dtype, device=y.device)
-    with _on(y.device):
-        _lib.call("kmc_combine", y.data_ptr(), _DTYPES[y.dtype], T, k, y.shape[1], slot.data_ptr(), _ptr(weights),
-                  out.data_ptr(), _stream())
+    _run("kmc_combine", y.device, y.data_ptr(), _DTYPES[y.dtype], T, k, y.shape[1], slot.data_ptr(), _ptr(weights),
+         out.data_ptr())
     return out
 
 
@@ -343,9 +337,8 @@ def _combine_grad(dout, y, groups, weights):
     T, k = slot.shape[0], (slot.shape[1] if slot.ndim == 2 else 1)
     dy = torch.empty_like(y)
     dw = torch.empty_like(weights) if weights is not None else None
-    with _on(y.device):
-        _lib.call("kmc_combine_grad", dout.data_ptr(), y.data_ptr(), _DTYPES[y.dtype], T, k, y.shape[1],
-                  slot.data_ptr(), _ptr(weights), groups.offsets[-1:].data_ptr(), dy.data_ptr(), _ptr(dw), _stream())
+    _run("kmc_combine_grad", y.device, dout.data_ptr(), y.data_ptr(), _DTYPES[y.dtype], T, k, y.shape[1],
+         slot.data_ptr(), _ptr(weights), groups.offsets.data_ptr() + 4 * (groups.offsets.numel() - 1), dy.data_ptr(), _ptr(dw))
     return dy, dw
 
 
