@@ -228,10 +228,17 @@ __device__ __forceinline__ void store_features(T* dst, int64_t ldo, int left, in
                 *reinterpret_cast<uint4*>(dst + r * ldo + g * 8) = *reinterpret_cast<const uint4*>(stash + r * 80 + g * 16);
         }
         __syncwarp();
-    } else if (lane < feats) {
+    } else {                                               // rows of any alignment: a row's 32 elements at a time
+        T* mine = reinterpret_cast<T*>(stash + lane * 66);
 #pragma unroll
-        for (int j = 0; j < 32; j++)
-            if (j < left) dst[lane * ldo + j] = Elem<T>::from(v[j]);
+        for (int j = 0; j < 32; j++) mine[j] = Elem<T>::from(v[j]);
+        __syncwarp();
+        if (lane < left) {
+#pragma unroll 8
+            for (int r = 0; r < 32; r++)
+                if (r < feats) dst[r * ldo + lane] = reinterpret_cast<const T*>(stash + r * 66)[lane];
+        }
+        __syncwarp();
     }
 }
 

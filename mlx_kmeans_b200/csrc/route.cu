@@ -13,10 +13,9 @@
 //   softmax  dl_i = p_i ([i chosen] g_i - sum_j g_j p_j) over the available, RENORM: over the chosen, 0 elsewhere
 //   sigmoid  dl_i = g_i s_i (1 - s_i), RENORM: (g_i - sum_j g_j s_j / S) / S  s_i (1 - s_i), S = sum of the chosen s_j
 //
-// One warp owns a row: lane L holds the PER consecutive experts from L PER on (PER = 1, 2, 4 .. 32: E up to 1024),
-// read with 16-byte loads where the row allows, as order-preserving 32-bit integers (0: not available).  A choice is
-// one redux.max over the lanes' best, a ballot whose first lane has the lowest index, and a rescan by that lane.
-// Memory or launch bound: E reads and 8 k bytes written per row.
+// LANES lanes of a warp own a row: lane L holds the PER consecutive experts from L PER on (E up to LANES PER), read
+// with 16-byte loads where the row allows, their keys as order-preserving 32-bit integers (0: not available).
+// E reads and 8 k bytes written per row are little; the choices' instructions bound it (see choose).
 #include "common.cuh"
 #include "experts.cuh"
 #include "kmc_internal.h"
@@ -38,23 +37,44 @@ __device__ __forceinline__ float unordered(unsigned u) {
 }
 __device__ __forceinline__ float sigmoid32(float l) { return __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-l))); }
 
-__device__ __forceinline__ float warp_sum(float v) {
+// Over the LANES lanes that share a row (aligned in the warp); every lane of the warp calls them.
+template <int LANES>
+__device__ __forceinline__ float row_sum(float v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+    for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
     return v;
 }
-__device__ __forceinline__ float warp_max(float v) {
+template <int LANES>
+__device__ __forceinline__ float row_max(float v) {        // a NaN only if every lane's is
+    if constexpr (LANES == 32) {
+        float m;
+        asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+        return m;
+    }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
+    for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
     return v;
+}
+template <int LANES>
+__device__ __forceinline__ unsigned row_max(unsigned v) {
+    if constexpr (LANES == 32) return __reduce_max_sync(kFull, v);
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(kFull, v, o));
+    return v;
+}
+template <int LANES>
+__device__ __forceinline__ unsigned row_ballot(bool p) {   // bit i: lane i of the row
+    const unsigned m = __ballot_sync(kFull, p);
+    if constexpr (LANES == 32) return m;
+    return (m >> (threadIdx.x & 31 & ~(LANES - 1))) & ((1u << (LANES & 31)) - 1u);
 }
 
 // The lane's PER logits of one row (-inf past the last expert).  vec: the row starts on a 16-byte boundary, or on
 // one of PER elements where that is less.
 template <typename T, int PER>
-__device__ __forceinline__ void load_row(const T* row, int experts, bool vec, float (&l)[PER]) {
+__device__ __forceinline__ void load_row(const T* row, int lane, int experts, bool vec, float (&l)[PER]) {
     constexpr int V = PER * sizeof(T) >= 16 ? 16 / sizeof(T) : PER;
-    const int i0 = (threadIdx.x & 31) * PER;
+    const int i0 = lane * PER;
 #pragma unroll
     for (int i = 0; i < PER; i += V) {
         if (vec && i0 + i + V <= experts) {
@@ -137,53 +157,24 @@ __device__ __forceinline__ void keep_groups(const RouteArgs& a, unsigned (&key)[
     }
 }
 
-template <typename T, int PER>
-__global__ void __launch_bounds__(kRouteWarps * 32)
-    k_route(const T* __restrict__ logits, RouteArgs a, int32_t* __restrict__ ids, float* __restrict__ weights) {
-    pdl_wait();
-    const int lane = threadIdx.x & 31;
-    const int64_t t = (int64_t)blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
-    if (t >= a.rows) return;
-    const T* row = logits + t * a.stride;
-    float l[PER];
-    load_row<T, PER>(row, a.experts, a.vec, l);
-    const bool live = a.mask == nullptr || a.mask[t] != 0;
-    unsigned key[PER];
-#pragma unroll
-    for (int i = 0; i < PER; i++) {
-        const int e = lane * PER + i;
-        float v = a.sigmoid ? sigmoid32(l[i]) : l[i];
-        if (a.bias != nullptr && e < a.experts) v = __fadd_rn(v, a.bias[e]);
-        key[i] = live && l[i] > -INFINITY && v > -INFINITY ? ordered(v) : 0u;
-    }
-    float m = 0.0f, total = 1.0f;
-    if (!a.sigmoid && !a.renorm) {                         // the softmax runs over every available logit
-        m = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < PER; i++) m = l[i] > m ? l[i] : m;
-        m = warp_max(m);
-        total = 0.0f;
-#pragma unroll
-        for (int i = 0; i < PER; i++) total += l[i] > -INFINITY ? expf(l[i] - m) : 0.0f;
-        total = warp_sum(total);
-    }
-    if (a.groups > 1) keep_groups<PER>(a, key);
-
+// The choices of one row by exact keys: lane j gets the j-th.  A choice is the maximum over the lanes' best keys, the
+// first lane that has it (the lowest index), and a rescan by that lane.
+template <int LANES, int PER>
+__device__ __noinline__ int choose_exact(unsigned (&key)[PER], int choices) {
+    const int lane = threadIdx.x & (LANES - 1);
     unsigned best = 0u;
-    int at = 0;
+    int at = 0, mine = -1;
 #pragma unroll
     for (int i = PER - 1; i >= 0; i--)
         if (key[i] >= best) {                              // the lowest of equal keys
             best = key[i];
             at = i;
         }
-    int mine = -1;                                         // lane j: the j-th choice
-    for (int j = 0; j < a.choices; j++) {
-        const unsigned top = __reduce_max_sync(kFull, best);
-        if (top == 0u) break;                              // nothing available is left
-        const int owner = __ffs(__ballot_sync(kFull, best == top)) - 1;
-        const int e = __shfl_sync(kFull, lane * PER + at, owner);
-        if (lane == j) mine = e;
+    for (int j = 0; j < choices; j++) {
+        const unsigned top = row_max<LANES>(best);
+        const int owner = __ffs(row_ballot<LANES>(best == top)) - 1;
+        const int e = __shfl_sync(kFull, lane * PER + at, owner, LANES);
+        if (lane == j && top != 0u) mine = e;              // 0: nothing available is left
         if (lane == owner) {
             best = 0u;
             const int gone = at;
@@ -197,37 +188,136 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
             }
         }
     }
+    return mine;
+}
+
+// The choices of one row.  Key and index share 32 bits: the key's upper bits, then the complement of the index, so one
+// maximum finds the best expert, lowest index first, and each lane's words are sorted once (min / max network) and
+// popped from the front.  The key's lowest bits are cut off for the index: where two neighbours in the order (the
+// first that is not chosen included) agree in all the bits that are left, the rows of the warp are decided by
+// choose_exact (`whole`: the cut bits say nothing, as for 16-bit logits without a bias, and equal words are equal keys).
+template <int LANES, int PER, bool HALF>
+__device__ __forceinline__ int choose(unsigned (&key)[PER], int choices, bool whole) {
+    constexpr unsigned INDEX = LANES * PER - 1;
+    const int lane = threadIdx.x & (LANES - 1);
+    unsigned w[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++) w[i] = key[i] ? (key[i] & ~INDEX) | (INDEX - (lane * PER + i)) : 0u;
+    auto order = [](unsigned& hi, unsigned& lo) {
+        const unsigned m = max(hi, lo);
+        lo = min(hi, lo);
+        hi = m;
+    };
+#pragma unroll
+    for (int size = 2; size <= PER; size *= 2) {           // bitonic, descending
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int j = i ^ (size - 1);
+            if (j > i) order(w[i], w[j]);
+        }
+#pragma unroll
+        for (int d = size / 4; d > 0; d /= 2)
+#pragma unroll
+            for (int i = 0; i < PER; i++)
+                if (!(i & d)) order(w[i], w[i + d]);
+    }
+    int mine = -1;
+    unsigned last = 0u;
+    bool close = false;
+    for (int j = 0; j < choices; j++) {
+        const unsigned top = row_max<LANES>(w[0]);
+        if (!(HALF && whole)) close |= top != 0u && ((top ^ last) & ~INDEX) == 0u;
+        last = top;
+        if (lane == j && top != 0u) mine = (int)(INDEX - (top & INDEX));   // 0: nothing available is left
+        if (w[0] == top) {
+#pragma unroll
+            for (int i = 0; i + 1 < PER; i++) w[i] = w[i + 1];
+            w[PER - 1] = 0u;
+        }
+    }
+    if (!(HALF && whole)) {
+        const unsigned top = row_max<LANES>(w[0]);         // the first that is not chosen
+        close |= top != 0u && ((top ^ last) & ~INDEX) == 0u;
+        if (__any_sync(kFull, close)) mine = choose_exact<LANES, PER>(key, choices);
+    }
+    return mine;
+}
+
+template <typename T, int LANES, int PER>
+__global__ void __launch_bounds__(kRouteWarps * 32)
+    k_route(const T* __restrict__ logits, RouteArgs a, int32_t* __restrict__ ids, float* __restrict__ weights) {
+    pdl_wait();
+    const int lane = threadIdx.x & (LANES - 1);
+    const int64_t slot = (int64_t)blockIdx.x * (kRouteWarps * 32 / LANES) + threadIdx.x / LANES;
+    const bool here = slot < a.rows;                       // lanes past the last row go along with it, and store nothing
+    const int64_t t = here ? slot : a.rows - 1;
+    const T* row = logits + t * a.stride;
+    float l[PER];
+    load_row<T, PER>(row, lane, a.experts, a.vec, l);
+    const bool live = a.mask == nullptr || a.mask[t] != 0;
+    float v[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++) v[i] = l[i];
+    if (a.sigmoid) {
+#pragma unroll
+        for (int i = 0; i < PER; i++) v[i] = sigmoid32(l[i]);
+    }
+    if (a.bias != nullptr) {
+#pragma unroll
+        for (int i = 0; i < PER; i++)
+            if (lane * PER + i < a.experts) v[i] = __fadd_rn(v[i], __ldg(a.bias + lane * PER + i));
+    }
+    unsigned key[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++) key[i] = live && l[i] > -INFINITY && v[i] > -INFINITY ? ordered(v[i]) : 0u;
+    float m = 0.0f, total = 1.0f;
+    if (!a.sigmoid && !a.renorm) {                         // the softmax runs over every available logit
+        m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < PER; i++) m = l[i] > m ? l[i] : m;
+        m = row_max<LANES>(m);
+        total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PER; i++) total += l[i] > -INFINITY ? expf(l[i] - m) : 0.0f;
+        total = row_sum<LANES>(total);
+    }
+    if constexpr (LANES == 32) {
+        if (a.groups > 1) keep_groups<PER>(a, key);
+    }
+
+    const int mine = choose<LANES, PER, sizeof(T) == 2>(key, a.choices, sizeof(T) == 2 && !a.sigmoid && a.bias == nullptr);
     float w = 0.0f;
     const bool got = mine >= 0;
     const float lm = got ? Elem<T>::to(row[mine]) : -INFINITY;
     if (a.sigmoid) {
         const float s = got ? sigmoid32(lm) : 0.0f;
         if (a.renorm) {
-            const float sum = warp_sum(s);
+            const float sum = row_sum<LANES>(s);
             w = sum > 0.0f ? s / sum : 0.0f;
         } else {
             w = s;
         }
     } else {
-        if (a.renorm) m = warp_max(lm);
+        if (a.renorm) m = row_max<LANES>(lm);
         const float p = got ? expf(lm - m) : 0.0f;
-        if (a.renorm) total = warp_sum(p);
+        if (a.renorm) total = row_sum<LANES>(p);
         w = got ? p / total : 0.0f;
     }
-    if (lane < a.choices) {
+    if (here && lane < a.choices) {
         ids[t * a.choices + lane] = mine;
         weights[t * a.choices + lane] = a.scale * w;
     }
 }
 
-template <typename T, int PER>
+template <typename T, int LANES, int PER>
 __global__ void __launch_bounds__(kRouteWarps * 32)
     k_route_grad(const float* __restrict__ dweights, const T* __restrict__ logits, const int32_t* __restrict__ ids,
                  RouteArgs a, T* __restrict__ dlogits) {
     pdl_wait();
-    const int lane = threadIdx.x & 31;
-    const int64_t t = (int64_t)blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
-    if (t >= a.rows) return;
+    const int lane = threadIdx.x & (LANES - 1);
+    const int64_t slot = (int64_t)blockIdx.x * (kRouteWarps * 32 / LANES) + threadIdx.x / LANES;
+    const bool here = slot < a.rows;                       // lanes past the last row go along with it, and store nothing
+    const int64_t t = here ? slot : a.rows - 1;
     const T* row = logits + t * a.stride;
     T* out = dlogits + t * a.experts;
     int id = lane < a.choices ? ids[t * a.choices + lane] : -1;
@@ -243,35 +333,35 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
         p = s;
         dot = 0.0f;
         if (a.renorm) {
-            total = warp_sum(s);
-            dot = total > 0.0f ? warp_sum(g * s) / total : 0.0f;
+            total = row_sum<LANES>(s);
+            dot = total > 0.0f ? row_sum<LANES>(g * s) / total : 0.0f;
         }
     } else if (a.renorm) {
-        m = warp_max(lm);
+        m = row_max<LANES>(lm);
         p = got ? expf(lm - m) : 0.0f;
-        total = warp_sum(p);
+        total = row_sum<LANES>(p);
         p = got ? p / total : 0.0f;
-        dot = warp_sum(g * p);
+        dot = row_sum<LANES>(g * p);
     }
     float dl[PER];
 #pragma unroll
     for (int i = 0; i < PER; i++) dl[i] = 0.0f;
     if (!a.sigmoid && !a.renorm) {
-        load_row<T, PER>(row, a.experts, a.vec, dl);
+        load_row<T, PER>(row, lane, a.experts, a.vec, dl);
         m = -INFINITY;
 #pragma unroll
         for (int i = 0; i < PER; i++) m = dl[i] > m ? dl[i] : m;
-        m = warp_max(m);
+        m = row_max<LANES>(m);
         total = 0.0f;
 #pragma unroll
         for (int i = 0; i < PER; i++) {
             dl[i] = dl[i] > -INFINITY ? expf(dl[i] - m) : 0.0f;
             total += dl[i];
         }
-        total = warp_sum(total);
+        total = row_sum<LANES>(total);
         p = got ? expf(lm - m) / total : 0.0f;
-        dot = warp_sum(g * p);
-        const float c = __any_sync(kFull, got) ? -dot / total : 0.0f;   // a row with no choice: 0, whatever its logits
+        dot = row_sum<LANES>(g * p);
+        const float c = row_ballot<LANES>(got) != 0u ? -dot / total : 0.0f;   // a row with no choice: 0, whatever its logits
 #pragma unroll
         for (int i = 0; i < PER; i++) dl[i] = dl[i] != 0.0f ? c * dl[i] : 0.0f;
     }
@@ -280,7 +370,8 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
     const int i0 = lane * PER;
 #pragma unroll
     for (int i = 0; i < PER; i += V) {
-        if (a.out_vec && i0 + i + V <= a.experts) {
+        if (!here) {
+        } else if (a.out_vec && i0 + i + V <= a.experts) {
             Pack<T, V> q;
 #pragma unroll
             for (int j = 0; j < V; j++) q.v[j] = Elem<T>::from(dl[i + j]);
@@ -292,7 +383,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
         }
     }
     __syncwarp();
-    if (got) {
+    if (here && got) {
         float v;
         if (a.sigmoid) {
             v = !a.renorm ? g * slope : total > 0.0f ? (g - dot) / total * slope : 0.0f;
@@ -303,20 +394,21 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
     }
 }
 
-template <typename T, int PER>
-cudaError_t run_route(const RouteCall& c, const RouteArgs& a, cudaStream_t st) {
-    const int64_t blocks = (a.rows + kRouteWarps - 1) / kRouteWarps;
+template <typename T, int LANES, int PER>
+cudaError_t run_route(const RouteCall& c, RouteArgs a, cudaStream_t st) {
+    const int64_t rows = kRouteWarps * 32 / LANES, blocks = (a.rows + rows - 1) / rows;
+    const size_t step = PER * sizeof(T) >= 16 ? 16 : PER * sizeof(T);
+    a.vec = reinterpret_cast<uintptr_t>(c.logits) % step == 0 && (c.stride * sizeof(T)) % step == 0;
+    a.out_vec = reinterpret_cast<uintptr_t>(c.dlogits) % step == 0 && (c.experts * sizeof(T)) % step == 0;
     if (c.dweights == nullptr)
-        return launch_pdl(k_route<T, PER>, dim3((unsigned)blocks), dim3(kRouteWarps * 32), 0, st,
+        return launch_pdl(k_route<T, LANES, PER>, dim3((unsigned)blocks), dim3(kRouteWarps * 32), 0, st,
                           static_cast<const T*>(c.logits), a, c.ids_out, c.weights);
-    return launch_pdl(k_route_grad<T, PER>, dim3((unsigned)blocks), dim3(kRouteWarps * 32), 0, st, c.dweights,
+    return launch_pdl(k_route_grad<T, LANES, PER>, dim3((unsigned)blocks), dim3(kRouteWarps * 32), 0, st, c.dweights,
                       static_cast<const T*>(c.logits), c.ids, a, static_cast<T*>(c.dlogits));
 }
 
 template <typename T>
 cudaError_t run_route_type(const RouteCall& c, cudaStream_t st) {
-    int per = 1;
-    while (per * 32 < c.experts) per *= 2;
     RouteArgs a;
     a.rows = c.rows;
     a.stride = c.stride;
@@ -330,17 +422,17 @@ cudaError_t run_route_type(const RouteCall& c, cudaStream_t st) {
     a.scale = c.scale;
     a.sigmoid = c.sigmoid;
     a.renorm = c.renorm;
-    const size_t step = per * sizeof(T) >= 16 ? 16 : per * sizeof(T);
-    a.vec = reinterpret_cast<uintptr_t>(c.logits) % step == 0 && (c.stride * sizeof(T)) % step == 0;
-    a.out_vec = reinterpret_cast<uintptr_t>(c.dlogits) % step == 0 && (c.experts * sizeof(T)) % step == 0;
-    switch (per) {
-        case 1: return run_route<T, 1>(c, a, st);
-        case 2: return run_route<T, 2>(c, a, st);
-        case 4: return run_route<T, 4>(c, a, st);
-        case 8: return run_route<T, 8>(c, a, st);
-        case 16: return run_route<T, 16>(c, a, st);
-        default: return run_route<T, 32>(c, a, st);
-    }
+    // Eight or sixteen lanes a row where its experts fit and its choices do (lane j holds the j-th): the work that is
+    // done once a row is then shared by four or two rows.  Groups of experts are compared across a whole warp.
+    if (c.groups <= 1 && c.experts <= 64 && c.choices <= 8)
+        return c.experts <= 32 ? run_route<T, 8, 4>(c, a, st) : run_route<T, 8, 8>(c, a, st);
+    if (c.groups <= 1 && c.experts <= 128 && c.choices <= 16) return run_route<T, 16, 8>(c, a, st);
+    if (c.experts <= 32) return run_route<T, 32, 1>(c, a, st);
+    if (c.experts <= 64) return run_route<T, 32, 2>(c, a, st);
+    if (c.experts <= 128) return run_route<T, 32, 4>(c, a, st);
+    if (c.experts <= 256) return run_route<T, 32, 8>(c, a, st);
+    if (c.experts <= 512) return run_route<T, 32, 16>(c, a, st);
+    return run_route<T, 32, 32>(c, a, st);
 }
 
 }  // namespace
