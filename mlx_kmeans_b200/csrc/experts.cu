@@ -21,6 +21,15 @@ constexpr int kTakeThreads = 256;
 bool readable(const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; }
 int64_t padded(int64_t cols) { return (cols + 7) / 8 * 8; }
 size_t a256(size_t v) { return (v + 255) & ~size_t(255); }
+// Forward products of few rows take expert_rows.cu: up to four rows an expert at any size, up to sixteen where all the
+// matrices together are small and the tensor-core kernel's set-up counts (device time, 16-bit, rows against tiles:
+// 2048 x 2048, 8 of 64 experts: 1 row each 16 us against 19, 4 each 94 against 95, 16 each 225 against 111;
+// 512 x 512, 8 experts: 1 to 4 rows each 3 us against 8, 16 each 5 against 9, 32 each 10 against 10).
+bool by_rows(const ExpertCall& c) {
+    if (c.kind != kExpertForward) return false;
+    const int64_t used = c.pairs < c.experts ? c.pairs : c.experts;
+    return c.pairs <= 4 * used || (c.pairs <= 16 * used && used * c.n * c.d <= (8 << 20));
+}
 bool takes_x(const ExpertCall& c) { return c.x && c.rows && !(c.kind == kExpertForward && expert_few_rows(c)); }
 
 // dst row i (cols elements, ldp apart) = src row idx[i], or row i without idx; zeros for a row outside src and in the
@@ -72,6 +81,7 @@ bool expert_few_rows(const ExpertCall& c) { return c.pairs <= (int64_t)c.experts
 
 size_t expert_bytes(const ExpertCall& c) {
     size_t need = 0;
+    if (by_rows(c)) return 0;
     if (takes_x(c)) need += a256((size_t)c.pairs * padded(c.d) * 2);
     else if (c.x && !readable(c.x, c.ldx)) need += a256((size_t)c.x_rows * padded(c.d) * 2);
     if (c.w && !readable(c.w, c.d)) need += a256((size_t)c.experts * c.n * padded(c.d) * 2);
@@ -84,6 +94,7 @@ cudaError_t launch_expert(const ExpertCall& c, cudaStream_t st) {
         return c.kind == kExpertForward ? cudaMemsetAsync(c.y, 0, (size_t)c.pairs * c.n * 2, st)
                                         : cudaMemsetAsync(c.dw, 0, (size_t)c.experts * c.n * c.d * 2, st);
     if (c.pairs == 0) return cudaMemsetAsync(c.dw, 0, (size_t)c.experts * c.n * c.d * 2, st);
+    if (by_rows(c)) return launch_expert_rows(c, st);
     Operands o = {c.x, c.w, c.dy, c.ldx, c.d, c.n, c.rows, c.x_rows};
     char* ws = static_cast<char*>(c.ws);
     cudaError_t e = cudaSuccess;

@@ -298,6 +298,9 @@ struct Operands {
     int64_t x_rows;
 };
 bool expert_few_rows(const ExpertCall& c);
+// forward products of a few rows (expert_rows.cu), on the operands as the caller gave them
+
+cudaError_t launch_expert_rows(const ExpertCall& c, cudaStream_t st);
 cudaError_t launch_expert_tc(const ExpertCall& c, const Operands& o, cudaStream_t st);
 
 }  // namespace kmc
