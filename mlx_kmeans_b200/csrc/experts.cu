@@ -17,6 +17,7 @@ namespace kmc {
 namespace {
 
 constexpr int kTakeThreads = 256;
+constexpr int kPieces = 4;
 
 bool readable(const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; }
 int64_t padded(int64_t cols) { return (cols + 7) / 8 * 8; }
@@ -33,45 +34,75 @@ bool by_rows(const ExpertCall& c) {
 bool takes_x(const ExpertCall& c) { return c.x && c.rows && !(c.kind == kExpertForward && expert_few_rows(c)); }
 
 // dst row i (cols elements, ldp apart) = src row idx[i], or row i without idx; zeros for a row outside src and in the
-// padding.  A thread writes 16 bytes; it reads them as one (VEC) or element by element.
-template <bool VEC>
-__global__ void __launch_bounds__(kTakeThreads)
-    k_take(const uint16_t* __restrict__ src, int64_t src_rows, const int32_t* __restrict__ idx, int64_t rows, int cols,
-           int64_t ld, int ldp, uint16_t* __restrict__ dst) {
+// padding
+struct Take {
+    const uint16_t* src;
+    int64_t src_rows, ld, rows;
+    const int32_t* idx;
+    int cols, ldp, vec;                   // vec: rows of src can be read 16 bytes at a time
+    uint16_t* dst;
+};
+
+// One or two copies in a launch (blockIdx.y): a thread writes kPieces times 16 bytes, read as one or element by element.
+__global__ void __launch_bounds__(kTakeThreads) k_take(Take t0, Take t1) {
     pdl_wait();
-    const int vecs = ldp / 8;
-    const int64_t i = (int64_t)blockIdx.x * kTakeThreads + threadIdx.x;
-    if (i >= rows * vecs) return;
-    const int64_t r = i / vecs;
-    const int c = (int)(i - r * vecs) * 8;
-    const int64_t s = idx ? (int64_t)__ldg(idx + r) : r;
-    Pack<uint16_t, 8> p = {};
-    if (s >= 0 && s < src_rows) {
-        if constexpr (VEC) {
-            p = *reinterpret_cast<const Pack<uint16_t, 8>*>(src + s * ld + c);
+    const Take& t = blockIdx.y == 0 ? t0 : t1;
+    const int vecs = t.ldp / 8;
+    const int64_t i0 = (int64_t)blockIdx.x * kTakeThreads * kPieces + threadIdx.x, all = t.rows * vecs;
+    Pack<uint16_t, 8> p[kPieces];
+#pragma unroll
+    for (int q = 0; q < kPieces; q++) {
+        const int64_t i = i0 + q * kTakeThreads;
+        p[q] = {};
+        if (i >= all) continue;
+        const int64_t r = i / vecs;
+        const int c = (int)(i - r * vecs) * 8;
+        const int64_t s = t.idx ? (int64_t)__ldg(t.idx + r) : r;
+        if (s < 0 || s >= t.src_rows) continue;
+        if (t.vec) {
+            p[q] = *reinterpret_cast<const Pack<uint16_t, 8>*>(t.src + s * t.ld + c);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                if (c + j < cols) p.v[j] = src[s * ld + c + j];
+                if (c + j < t.cols) p[q].v[j] = t.src[s * t.ld + c + j];
         }
     }
-    *reinterpret_cast<Pack<uint16_t, 8>*>(dst + r * ldp + c) = p;
+#pragma unroll
+    for (int q = 0; q < kPieces; q++) {
+        const int64_t i = i0 + q * kTakeThreads;
+        if (i < all) *reinterpret_cast<Pack<uint16_t, 8>*>(t.dst + i * 8) = p[q];
+    }
 }
 
-// Replaces the operand at *p by its copy in the workspace
-cudaError_t take(const void** p, int64_t* ld, int64_t src_rows, const int32_t* idx, int64_t rows, int cols, char** ws,
-                 cudaStream_t st) {
-    const int64_t ldp = padded(cols), blocks = (rows * (ldp / 8) + kTakeThreads - 1) / kTakeThreads;
-    if (blocks >= INT32_MAX) return cudaErrorInvalidValue;
-    const bool vec = readable(*p, *ld) && cols % 8 == 0;
-    cudaError_t e = launch_pdl(vec ? k_take<true> : k_take<false>, dim3((unsigned)blocks), dim3(kTakeThreads), 0, st,
-                               static_cast<const uint16_t*>(*p), src_rows, idx, rows, cols, *ld, (int)ldp,
-                               reinterpret_cast<uint16_t*>(*ws));
-    *p = *ws;
-    *ld = ldp;
-    *ws += a256((size_t)rows * ldp * 2);
-    return e;
-}
+// The copies of one call, in the workspace
+struct Takes {
+    Take t[2] = {};
+    int n = 0;
+    char* ws;
+    void add(const void** p, int64_t* ld, int64_t src_rows, const int32_t* idx, int64_t rows, int cols) {
+        Take& k = t[n++];
+        k.src = static_cast<const uint16_t*>(*p);
+        k.src_rows = src_rows;
+        k.ld = *ld;
+        k.rows = rows;
+        k.idx = idx;
+        k.cols = cols;
+        k.ldp = (int)padded(cols);
+        k.vec = readable(*p, *ld) && cols % 8 == 0;
+        k.dst = reinterpret_cast<uint16_t*>(ws);
+        *p = ws;
+        *ld = k.ldp;
+        ws += a256((size_t)rows * k.ldp * 2);
+    }
+    cudaError_t launch(cudaStream_t st) const {
+        if (n == 0) return cudaSuccess;
+        int64_t most = 1;
+        for (int i = 0; i < n; i++) most = t[i].rows * (t[i].ldp / 8) > most ? t[i].rows * (t[i].ldp / 8) : most;
+        const int64_t blocks = (most + kTakeThreads * kPieces - 1) / (kTakeThreads * kPieces);
+        if (blocks >= INT32_MAX) return cudaErrorInvalidValue;
+        return launch_pdl(k_take, dim3((unsigned)blocks, n), dim3(kTakeThreads), 0, st, t[0], t[1]);
+    }
+};
 
 }  // namespace
 
@@ -96,21 +127,19 @@ cudaError_t launch_expert(const ExpertCall& c, cudaStream_t st) {
     if (c.pairs == 0) return cudaMemsetAsync(c.dw, 0, (size_t)c.experts * c.n * c.d * 2, st);
     if (by_rows(c)) return launch_expert_rows(c, st);
     Operands o = {c.x, c.w, c.dy, c.ldx, c.d, c.n, c.rows, c.x_rows};
-    char* ws = static_cast<char*>(c.ws);
-    cudaError_t e = cudaSuccess;
+    Takes copies;
+    copies.ws = static_cast<char*>(c.ws);
     if (takes_x(c)) {
-        e = take(&o.x, &o.ldx, c.x_rows, c.rows, c.pairs, c.d, &ws, st);
+        copies.add(&o.x, &o.ldx, c.x_rows, c.rows, c.pairs, c.d);
         o.rows = nullptr;
         o.x_rows = c.pairs;
     } else if (o.x && !readable(o.x, o.ldx)) {
-        e = take(&o.x, &o.ldx, c.x_rows, nullptr, c.x_rows, c.d, &ws, st);
+        copies.add(&o.x, &o.ldx, c.x_rows, nullptr, c.x_rows, c.d);
     }
-    if (e == cudaSuccess && o.w && !readable(o.w, o.ldw)) {
-        const int64_t rows = (int64_t)c.experts * c.n;
-        e = take(&o.w, &o.ldw, rows, nullptr, rows, c.d, &ws, st);
-    }
-    if (e == cudaSuccess && o.dy && !readable(o.dy, o.lddy)) e = take(&o.dy, &o.lddy, c.pairs, nullptr, c.pairs, c.n, &ws, st);
-    return e == cudaSuccess ? launch_expert_tc(c, o, st) : e;
+    if (o.w && !readable(o.w, o.ldw)) copies.add(&o.w, &o.ldw, (int64_t)c.experts * c.n, nullptr, (int64_t)c.experts * c.n, c.d);
+    if (o.dy && !readable(o.dy, o.lddy)) copies.add(&o.dy, &o.lddy, c.pairs, nullptr, c.pairs, c.n);
+    if (cudaError_t e = copies.launch(st)) return e;
+    return launch_expert_tc(c, o, st);
 }
 
 }  // namespace kmc

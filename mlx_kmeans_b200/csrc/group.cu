@@ -21,7 +21,10 @@ namespace {
 constexpr int kGroupThreads = 1024;
 constexpr int kGroupWarps = kGroupThreads / 32;
 constexpr int64_t kOneChunk = 8192;       // pairs one CTA takes by itself
-constexpr int64_t kChunkMin = 4096;       // pairs per chunk otherwise (more when there are more chunks than SMs)
+constexpr int64_t kChunkMin = 4096;       // pairs per chunk otherwise, more where that makes over kMaxChunks of them
+constexpr int kMaxChunks = 148;           // one per SM
+constexpr int kChunkLoads = (kMaxChunks + 31) / 32;
+constexpr int kAhead = 8;                 // ids a thread has in flight
 constexpr int kCounters = 32768;          // per-warp counters in shared memory (128 KB): fewer warps work above 1024 experts
 
 struct GroupArgs {
@@ -40,9 +43,16 @@ __global__ void __launch_bounds__(kGroupThreads) k_group_count(GroupArgs a) {
     for (int e = threadIdx.x; e < a.experts; e += kGroupThreads) count[e] = 0;
     __syncthreads();
     const int64_t p0 = (int64_t)blockIdx.x * a.chunk, p1 = min(p0 + a.chunk, a.pairs);
-    for (int64_t p = p0 + threadIdx.x; p < p1; p += kGroupThreads) {
-        const int e = __ldg(a.ids + p);
-        if (e >= 0 && e < a.experts) atomicAdd(count + e, 1);
+    for (int64_t b = p0; b < p1; b += kAhead * kGroupThreads) {
+        int e[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+            const int64_t p = b + j * kGroupThreads + threadIdx.x;
+            e[j] = p < p1 ? __ldg(a.ids + p) : -1;
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; j++)
+            if (e[j] >= 0 && e[j] < a.experts) atomicAdd(count + e[j], 1);
     }
     __syncthreads();
     for (int e = threadIdx.x; e < a.experts; e += kGroupThreads)
@@ -66,28 +76,48 @@ __global__ void __launch_bounds__(kGroupThreads) k_group_place(GroupArgs a, int 
     const int64_t p0 = (int64_t)blockIdx.x * a.chunk, p1 = min(p0 + a.chunk, a.pairs);
     const int64_t per = ((p1 - p0 + warps - 1) / warps + 31) / 32 * 32;
     const int64_t w0 = min(p0 + warp * per, p1), w1 = warp < warps ? min(w0 + per, p1) : w0;
-    for (int64_t p = w0 + lane; p < w1; p += 32) {
-        const int e = __ldg(a.ids + p);
-        if (e >= 0 && e < E) atomicAdd(run + warp * E + e, 1);
+    int ids[kAhead];                      // 256 pairs of the run at a time
+    auto load = [&](int64_t b) {
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+            const int64_t p = b + j * 32 + lane;
+            const int e = p < w1 ? __ldg(a.ids + p) : -1;
+            ids[j] = e < 0 || e > E ? E : e;               // E: left out
+        }
+    };
+    for (int64_t b = w0; b < w1; b += kAhead * 32) {
+        load(b);
+#pragma unroll
+        for (int j = 0; j < kAhead; j++)
+            if (ids[j] < E) atomicAdd(run + warp * E + ids[j], 1);
     }
     if (a.chunks > 1) {
-        // a warp per expert: its counts of all chunks lie side by side, so its loads are independent (a thread per
-        // expert walking down the chunks waited for the L2 once per chunk: 34 us at 2^20 pairs of 256 experts)
-#pragma unroll 4
-        for (int e = warp; e < E; e += kGroupWarps) {
-            const int32_t* c = a.counts + (int64_t)e * a.chunks;
-            int32_t sum = 0, below = 0;
-#pragma unroll 5
-            for (int i = lane; i < a.chunks; i += 32) {
-                const int32_t v = __ldcg(c + i);
-                sum += v;
-                below += i < (int)blockIdx.x ? v : 0;
-            }
-            sum = __reduce_add_sync(0xffffffffu, sum);
-            below = __reduce_add_sync(0xffffffffu, below);
-            if (lane == 0) {
-                total[e] = sum;
-                before[e] = below;
+        // a warp per expert, four at a time: the counts of all chunks lie side by side and are in flight together (a
+        // thread per expert walking down the chunks waited for the L2 once a chunk, 10 us more at 2^20 pairs)
+        for (int e0 = warp; e0 < E; e0 += 4 * kGroupWarps) {
+            int32_t v[4][kChunkLoads];
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+#pragma unroll
+                for (int i = 0; i < kChunkLoads; i++) {
+                    const int e = e0 + q * kGroupWarps, c = i * 32 + lane;
+                    v[q][i] = e < E && c < a.chunks ? __ldcg(a.counts + (int64_t)e * a.chunks + c) : 0;
+                }
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const int e = e0 + q * kGroupWarps;
+                int32_t sum = 0, below = 0;
+#pragma unroll
+                for (int i = 0; i < kChunkLoads; i++) {
+                    sum += v[q][i];
+                    below += i * 32 + lane < (int)blockIdx.x ? v[q][i] : 0;
+                }
+                sum = __reduce_add_sync(0xffffffffu, sum);
+                below = __reduce_add_sync(0xffffffffu, below);
+                if (lane == 0 && e < E) {
+                    total[e] = sum;
+                    before[e] = below;
+                }
             }
         }
         __syncthreads();
@@ -128,12 +158,15 @@ __global__ void __launch_bounds__(kGroupThreads) k_group_place(GroupArgs a, int 
         base += warp_total[kGroupWarps - 1];
         if (e < E) {
             if (blockIdx.x == 0) a.offsets[e] = start;
-            int32_t next = start + before[e];
-            for (int w = 0; w < warps; w++) {
-                const int32_t n = run[w * E + e];
-                run[w * E + e] = next;
-                next += n;
-            }
+            int32_t next = start + before[e], n[kGroupWarps];
+#pragma unroll
+            for (int w = 0; w < kGroupWarps; w++) n[w] = w < warps ? run[w * E + e] : 0;
+#pragma unroll
+            for (int w = 0; w < kGroupWarps; w++)
+                if (w < warps) {
+                    run[w * E + e] = next;
+                    next += n[w];
+                }
         }
         __syncthreads();
     }
@@ -144,26 +177,30 @@ __global__ void __launch_bounds__(kGroupThreads) k_group_place(GroupArgs a, int 
     __syncthreads();
 
     const int bits = 32 - __clz(E);
-    for (int64_t b = w0; b < w1; b += 32) {
-        const int64_t p = b + lane;
-        int e = p < w1 ? __ldg(a.ids + p) : -1;
-        if (e < 0 || e >= E) e = E;
-        // the lanes of the same expert, one ballot per bit of the index (match.any took ten times the instructions)
-        unsigned same = 0xffffffffu;
-        for (int bit = 0; bit < bits; bit++) {
-            const bool one = (e >> bit) & 1;
-            const unsigned m = __ballot_sync(0xffffffffu, one);
-            same &= one ? m : ~m;
-        }
-        const int ahead = __popc(same & ((1u << lane) - 1u));
-        int32_t pos = -1;
-        if (e < E) pos = run[warp * E + e] + ahead;
-        __syncwarp();
-        if (e < E && ahead == 0) run[warp * E + e] = pos + __popc(same);
-        __syncwarp();
-        if (p < w1) {
-            a.slot[p] = pos;
-            if (e < E) a.rows[pos] = (int32_t)((uint32_t)p / (uint32_t)a.choices);
+    for (int64_t b0 = w0; b0 < w1; b0 += kAhead * 32) {
+        if (w1 - w0 > kAhead * 32) load(b0);               // (a shorter run is still in the registers)
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+            const int64_t b = b0 + j * 32, p = b + lane;
+            if (b >= w1) break;
+            const int e = ids[j];
+            // the lanes of the same expert, one ballot per bit of the index (match.any took ten times the instructions)
+            unsigned same = 0xffffffffu;
+            for (int bit = 0; bit < bits; bit++) {
+                const bool one = (e >> bit) & 1;
+                const unsigned m = __ballot_sync(0xffffffffu, one);
+                same &= one ? m : ~m;
+            }
+            const int ahead = __popc(same & ((1u << lane) - 1u));
+            int32_t pos = -1;
+            if (e < E) pos = run[warp * E + e] + ahead;
+            __syncwarp();
+            if (e < E && ahead == 0) run[warp * E + e] = pos + __popc(same);
+            __syncwarp();
+            if (p < w1) {
+                a.slot[p] = pos;
+                if (e < E) a.rows[pos] = (int32_t)((uint32_t)p / (uint32_t)a.choices);
+            }
         }
     }
     for (int64_t p = p0 + threadIdx.x; p < p1; p += kGroupThreads)
@@ -172,8 +209,8 @@ __global__ void __launch_bounds__(kGroupThreads) k_group_place(GroupArgs a, int 
 
 int64_t group_chunk(int64_t pairs) {
     if (pairs <= kOneChunk) return pairs > 0 ? pairs : 1;
-    const int64_t per_sm = (pairs + 147) / 148;
-    return per_sm > kChunkMin ? per_sm : kChunkMin;
+    const int64_t least = (pairs + kMaxChunks - 1) / kMaxChunks;
+    return least > kChunkMin ? least : kChunkMin;
 }
 
 }  // namespace
