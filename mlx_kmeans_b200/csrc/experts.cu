@@ -6,8 +6,10 @@
 //
 // Rows of x read by index: with few rows an expert the products' kernel gathers them itself (tile::gather4).  A gather
 // of four 128-byte pieces took 36 cycles of the TMA unit however it was issued, so a tile of 256 positions spent four
-// times as long on them as on its MMAs (8192 x 8 of 64 experts, 2048 x 2048: 2365 us, from grouped rows 529 us); with
-// many rows an expert, and for dW, they are copied in grouped order first.
+// times as long on them as on its MMAs (8192 x 8 of 64 experts, 2048 x 2048: 2365 us, from grouped rows 529 us), and
+// warps that gather with 16-byte asynchronous copies took 1190 us (the hand-over of a stage from copies to tensor cores
+// takes longer than its MMAs).  With many rows an expert, and for dW, x is copied in grouped order first: 70 us there,
+// what writing it takes, of 560 in all.
 #include "common.cuh"
 #include "experts.cuh"
 #include "kmc_internal.h"

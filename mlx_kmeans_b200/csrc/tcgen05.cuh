@@ -90,8 +90,10 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// An arrival on another CTA's barrier.  What it hands over is TMEM, which the tcgen05 fences order, and no ordinary
+// memory: so no release at cluster scope, whose memory barrier took most of a microsecond.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 // Four rows of a 2-D tensor by their indices, as four consecutive rows of the box (one row high in the map); a row
 // past the tensor's last is filled with zeros.
