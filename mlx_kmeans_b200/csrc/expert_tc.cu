@@ -52,6 +52,7 @@ struct TcArgs {
     int feats;                            // M side in all: n (forward, dW), d (dx)
     int cols;                             // dW: N side in all (d); otherwise unused
     int depth;                            // forward: d, dx: n; dW: per expert
+    int most;                             // positions per tile at most (forward, dx): COLS, or fewer (see run_tc)
     void* out;
     int64_t ldo;                          // row length of out
     int out_vec;                          // rows of out start on 16-byte boundaries
@@ -92,10 +93,10 @@ struct Shape {
     static constexpr int FEATS = PAIR ? 2 * kFeat : kFeat;    // features per tile
     static constexpr int STEP = PAIR ? 32 : 16;               // granularity of the MMA's N
 
-    static __device__ __forceinline__ int feature_tiles(const TcArgs& a) { return (a.feats + FEATS - 1) / FEATS; }
-    // Rows per tile of an expert with `count` rows: equal tiles of whole STEPs, at most COLS
-    static __device__ __forceinline__ int rows(int count) {
-        const int tiles = (count + COLS - 1) / COLS;
+    static __host__ __device__ __forceinline__ int feature_tiles(const TcArgs& a) { return (a.feats + FEATS - 1) / FEATS; }
+    // Rows per tile of an expert with `count` rows: equal tiles of whole STEPs, at most a.most
+    static __device__ __forceinline__ int rows(const TcArgs& a, int count) {
+        const int tiles = (count + a.most - 1) / a.most;
         return tiles == 0 ? COLS : ((count + tiles - 1) / tiles + STEP - 1) / STEP * STEP;
     }
     // Tiles of expert e per feature tile
@@ -103,7 +104,7 @@ struct Shape {
         if constexpr (MODE == kExpertDw) return (a.cols + COLS - 1) / COLS;
         int begin, count;
         segment(a, e, begin, count);
-        const int size = rows(count);
+        const int size = rows(a, count);
         return (count + size - 1) / size;
     }
     // Tile t; `e` walks up with t, first[e] = tiles of the experts before e.  An expert's tiles go in blocks of kBlock
@@ -127,7 +128,7 @@ struct Shape {
             r.ncols = min((a.cols - r.c0 + STEP - 1) / STEP * STEP, COLS);
             r.steps = (count + kDepth - 1) / kDepth;
         } else {
-            const int size = rows(count);
+            const int size = rows(a, count);
             r.c0 = 0;
             r.p0 = begin + tile * size;
             r.p1 = min(r.p0 + size, begin + count);
@@ -540,7 +541,7 @@ bool make_map(CUtensorMap* m, int dtype, const void* base, int64_t cols, int64_t
 }
 
 template <typename T, int MODE, int COLS, bool GATHER, bool PAIR>
-cudaError_t run_tc(const CUtensorMap (&m)[4], const TcArgs& a, cudaStream_t st) {
+cudaError_t run_tc(const CUtensorMap (&m)[4], TcArgs a, cudaStream_t st) {
     auto kern = k_expert_tc<T, MODE, COLS, GATHER, PAIR>;
     using S = TcSmem<COLS, PAIR>;
     static unsigned long long configured = 0;
@@ -553,6 +554,13 @@ cudaError_t run_tc(const CUtensorMap (&m)[4], const TcArgs& a, cudaStream_t st) 
     }
     const size_t smem = S::base + (size_t)(a.experts + 1) * 4;
     const int grid = PAIR ? num_sms() / 2 * 2 : num_sms();
+    // Fewer positions a tile where the results' rows are not on 16-byte boundaries, whose element-wise stores are most of
+    // a small call's time, and full tiles would leave CTAs without any: as many as give each CTA (or pair) one tile, 32
+    // at least (1554 rows of 12 experts, 515 x 333: 52.8 -> 47.5 us for y, dx and dW).  Not otherwise: every further
+    // tile reads its features' matrix again (597 rows of 8 experts, 1072 x 1800: 67.3 -> 75.6 us).
+    using Sh = Shape<MODE, COLS, PAIR>;
+    const int64_t share = (int64_t)a.pairs * Sh::feature_tiles(a) / (grid / (PAIR ? 2 : 1));
+    a.most = a.out_vec || share >= COLS ? COLS : share <= 32 ? 32 : (int)(share + 31) / 32 * 32;
     if constexpr (PAIR) return launch_pdl_clusters(kern, dim3(grid), dim3(kTcThreads), smem, st, 2, m[0], m[1], m[2], m[3], a);
     return launch_pdl(kern, dim3(grid), dim3(kTcThreads), smem, st, m[0], m[1], m[2], m[3], a);
 }
