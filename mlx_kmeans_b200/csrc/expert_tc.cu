@@ -101,26 +101,34 @@ struct Shape {
     }
     // Tiles of expert e per feature tile
     static __device__ __forceinline__ int tiles(const TcArgs& a, int e) {
-        if constexpr (MODE == kExpertDw) return (a.cols + COLS - 1) / COLS;
         int begin, count;
         segment(a, e, begin, count);
         const int size = rows(a, count);
         return (count + size - 1) / size;
     }
-    // Tile t; `e` walks up with t, first[e] = tiles of the experts before e.  An expert's tiles go in blocks of kBlock
+    // Tile t; `e` walks up with t, first[e] = tiles of the experts before e (dW: the e-th expert by size).  An expert's tiles go in blocks of kBlock
     // position tiles (dW: column tiles) by all feature tiles, positions fastest, so the tiles that run at the same time
     // read about as many rows of the one operand as of the other, and the L2 serves them.
     static __device__ __forceinline__ Tile at(const TcArgs& a, const int* first, int64_t t, int& e) {
         Tile r;
         const int ft = feature_tiles(a), j = (int)(t / ft);
-        while (j >= first[e + 1]) e++;
-        const int in = (int)(t - (int64_t)first[e] * ft), block = in / (kBlock * ft);
-        const int left = first[e + 1] - first[e] - block * kBlock, wide = left < kBlock ? left : kBlock;
+        int before, here;                                 // position tiles of the experts before, and of this one
+        if constexpr (MODE == kExpertDw) {
+            here = (a.cols + COLS - 1) / COLS;
+            before = j / here * here;
+            r.e = first[j / here];
+        } else {
+            while (j >= first[e + 1]) e++;
+            before = first[e];
+            here = first[e + 1] - before;
+            r.e = e;
+        }
+        const int in = (int)(t - (int64_t)before * ft), block = in / (kBlock * ft);
+        const int left = here - block * kBlock, wide = left < kBlock ? left : kBlock;
         const int k = in - block * kBlock * ft, tile = block * kBlock + k % wide;
         r.f0 = k / wide * FEATS;
-        r.e = e;
         int begin, count;
-        segment(a, e, begin, count);
+        segment(a, r.e, begin, count);
         if constexpr (MODE == kExpertDw) {
             r.c0 = tile * COLS;
             r.p0 = begin;
@@ -295,8 +303,34 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
     }
     pdl_wait();
-    // first[e]: tiles of the experts before e, by a scan over per-thread runs of experts
-    {
+    int64_t tiles;
+    if constexpr (MODE == kExpertDw) {
+        // first[i]: the i-th expert by number of rows, most first.  A tile's depth is its expert's rows, and the tiles
+        // go to the CTAs in turn: in that order each CTA gets about the same depth in all (in the order of the experts,
+        // 10976 rows of 32 experts, 576 x 1904: 63 us).  Beyond kSorted experts, in their own order.
+        constexpr int kSorted = 2 * kTcThreads;
+        int count[2] = {}, rank[2] = {}, begin;
+        for (int i = 0; i < 2; i++) {
+            const int x = threadIdx.x + i * kTcThreads;
+            if (x < a.experts && a.experts <= kSorted) {
+                segment(a, x, begin, count[i]);
+                first[x] = count[i];
+            }
+        }
+        __syncthreads();
+        if (a.experts <= kSorted)
+            for (int y = 0; y < a.experts; y++) {
+                const int c = first[y];
+                for (int i = 0; i < 2; i++) {
+                    const int x = threadIdx.x + i * kTcThreads;
+                    rank[i] += c > count[i] || (c == count[i] && y < x) ? 1 : 0;
+                }
+            }
+        __syncthreads();
+        for (int x = threadIdx.x, i = 0; x < a.experts; x += kTcThreads, i++) first[a.experts <= kSorted ? rank[i & 1] : x] = x;
+        tiles = (int64_t)a.experts * ((a.cols + COLS - 1) / COLS) * Sh::feature_tiles(a);
+    } else {
+        // first[e]: tiles of the experts before e, by a scan over per-thread runs of experts
         const int run = (a.experts + kTcThreads - 1) / kTcThreads, e0 = min((int)threadIdx.x * run, a.experts);
         const int e1 = min(e0 + run, a.experts);
         int sum = 0;
@@ -322,7 +356,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     else __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const int64_t tiles = (int64_t)first[a.experts] * Sh::feature_tiles(a);
+    if constexpr (MODE != kExpertDw) tiles = (int64_t)first[a.experts] * Sh::feature_tiles(a);
     const int64_t t0 = blockIdx.x / CTAS, dt = gridDim.x / CTAS;
     int e = 0;
 
@@ -565,11 +599,13 @@ cudaError_t run_tc(const CUtensorMap (&m)[4], TcArgs a, cudaStream_t st) {
     return launch_pdl(kern, dim3(grid), dim3(kTcThreads), smem, st, m[0], m[1], m[2], m[3], a);
 }
 
-// The pair's 256 features where there are more than 128; one CTA's 128 otherwise.
+// A pair's tiles of 256 features, or one CTA's of 128 where there are no more, or (forward, dx: 576 features 46 -> 36 us)
+// where those cover a tenth less that does not exist; a pair does the same work about a tenth faster.
 template <typename T, int MODE, int COLS, bool GATHER>
 cudaError_t run_shape(const CUtensorMap (&m)[4], const TcArgs& a, cudaStream_t st) {
     if constexpr (COLS == 256) {
-        if (a.feats > kFeat) return run_tc<T, MODE, COLS, GATHER, true>(m, a, st);
+        const int whole = (a.feats + 255) / 256 * 256, half = (a.feats + 127) / 128 * 128;
+        if (MODE == kExpertDw ? a.feats > kFeat : whole * 10 <= half * 11) return run_tc<T, MODE, COLS, GATHER, true>(m, a, st);
     }
     return run_tc<T, MODE, COLS, GATHER, false>(m, a, st);
 }
