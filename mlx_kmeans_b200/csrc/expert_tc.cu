@@ -59,6 +59,11 @@ struct TcArgs {
     int* error;
 };
 
+// Loads by index or of the end of a group: rows of x (GATHER), and for dW 16 rows and single rows of dy and x
+struct Tails {
+    CUtensorMap a16, a_row, b16, b_row;
+};
+
 template <int COLS, bool PAIR>
 struct TcSmem {
     static constexpr int MINE = PAIR ? COLS / 2 : COLS;       // columns whose operand this CTA holds
@@ -253,8 +258,8 @@ __device__ __forceinline__ void store_features(T* dst, int64_t ldo, int left, in
 
 template <typename T, int MODE, int COLS, bool GATHER, bool PAIR>
 __global__ void __launch_bounds__(kTcThreads, 1)
-    k_expert_tc(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap ma_row,
-                const __grid_constant__ CUtensorMap mb, const __grid_constant__ CUtensorMap mb_row, TcArgs a) {
+    k_expert_tc(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb,
+                const __grid_constant__ Tails tails, TcArgs a) {
     static_assert(!GATHER || (MODE == kExpertForward && !PAIR && COLS <= 128), "gathers: one per lane and stage");
     using S = TcSmem<COLS, PAIR>;
     using Sh = Shape<MODE, COLS, PAIR>;
@@ -387,25 +392,32 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const uint32_t sa = base + stage * S::STAGE, sb = sa + S::A;
                 const uint32_t bar = PAIR ? cluster_addr(full(stage), 0) : full(stage);
                 if constexpr (MODE == kExpertDw) {
-                    // A: dy, two boxes of 64 features x 64 positions; B: x, boxes of 64 columns.  The last positions of
-                    // a group are gathered, zeros past its end.
-                    const int k0 = w.p0 + kc * kDepth, nb = (half + 63) / 64, c0 = w.c0 + rank * half;
-                    if (lane == 0 && rank == 0) mbar_expect_tx(full(stage), (uint32_t)(CTAS * (2 + nb)) * kBox);
+                    // A: dy, two boxes of 64 features x 64 positions; B: x, boxes of 64 columns.  The last stage of a
+                    // group takes its positions 16 at a time, and the ones past its last whole 16 by gathers of four,
+                    // which give zeros past its end (a gather of four takes about as long as a box: the whole stage by
+                    // gathers took as long as three others)
+                    const int k0 = w.p0 + kc * kDepth, v = min(w.p1 - k0, kDepth), nb = (half + 63) / 64;
+                    const int c0 = w.c0 + rank * half;
+                    if (lane == 0 && rank == 0)
+                        mbar_expect_tx(full(stage), (uint32_t)(CTAS * (2 + nb)) * (uint32_t)((v + 15) / 16 * 16 * 128));
                     __syncwarp();
-                    if (k0 + kDepth <= w.p1) {
+                    if (v == kDepth) {
                         if (lane < 2) load_2d<PAIR>(sa + lane * kBox, &ma, f0 + lane * 64, k0, bar);
                         else if (lane < 2 + nb) load_2d<PAIR>(sb + (lane - 2) * kBox, &mb, c0 + (lane - 2) * 64, k0, bar);
                     } else {
-                        const int g = (lane & 15) * 4;
-                        int q[4], x[4];
+                        const int i = lane & 7, part = v / 16 * 16 + (i & 3) * 4;
+                        for (int h = lane >> 3; h < 2 + nb; h += 4) {
+                            const uint32_t to = h < 2 ? sa + h * kBox : sb + (h - 2) * kBox;
+                            const int col = h < 2 ? f0 + h * 64 : c0 + (h - 2) * 64;
+                            if (i < v / 16) {
+                                load_2d<PAIR>(to + i * 2048, h < 2 ? &tails.a16 : &tails.b16, col, k0 + i * 16, bar);
+                            } else if (i >= 4 && v % 16 != 0) {
+                                int q[4];                  // (x is in grouped order too)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            q[i] = k0 + g + i < w.p1 ? k0 + g + i : a.pairs;
-                            x[i] = gather_row(a, k0 + g + i, w.p1);
+                                for (int n = 0; n < 4; n++) q[n] = k0 + part + n < w.p1 ? k0 + part + n : a.pairs;
+                                gather4<PAIR>(to + part * 128, h < 2 ? &tails.a_row : &tails.b_row, col, q, bar);
+                            }
                         }
-                        gather4<PAIR>(sa + (lane >> 4) * kBox + g * 128, &ma_row, f0 + (lane >> 4) * 64, q, bar);
-                        for (int h = lane >> 4; h < nb; h += 2)
-                            gather4<PAIR>(sb + h * kBox + g * 128, &mb_row, c0 + h * 64, x, bar);
                     }
                 } else {
                     const int nb = GATHER ? half / 4 : (half + 31) / 32;
@@ -420,7 +432,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                     __syncwarp();
                     if (lane < nb) {
-                        if constexpr (GATHER) gather4<PAIR>(sb + lane * 512, &mb_row, kc * kDepth, r, bar);
+                        if constexpr (GATHER) gather4<PAIR>(sb + lane * 512, &tails.b_row, kc * kDepth, r, bar);
                         else load_2d<PAIR>(sb + lane * 4096, &mb, kc * kDepth, w.p0 + rank * half + lane * 32, bar);
                     }
                 }
@@ -575,7 +587,7 @@ bool make_map(CUtensorMap* m, int dtype, const void* base, int64_t cols, int64_t
 }
 
 template <typename T, int MODE, int COLS, bool GATHER, bool PAIR>
-cudaError_t run_tc(const CUtensorMap (&m)[4], TcArgs a, cudaStream_t st) {
+cudaError_t run_tc(const CUtensorMap (&m)[2], const Tails& tails, TcArgs a, cudaStream_t st) {
     auto kern = k_expert_tc<T, MODE, COLS, GATHER, PAIR>;
     using S = TcSmem<COLS, PAIR>;
     static unsigned long long configured = 0;
@@ -595,24 +607,25 @@ cudaError_t run_tc(const CUtensorMap (&m)[4], TcArgs a, cudaStream_t st) {
     using Sh = Shape<MODE, COLS, PAIR>;
     const int64_t share = (int64_t)a.pairs * Sh::feature_tiles(a) / (grid / (PAIR ? 2 : 1));
     a.most = a.out_vec || share >= COLS ? COLS : share <= 32 ? 32 : (int)(share + 31) / 32 * 32;
-    if constexpr (PAIR) return launch_pdl_clusters(kern, dim3(grid), dim3(kTcThreads), smem, st, 2, m[0], m[1], m[2], m[3], a);
-    return launch_pdl(kern, dim3(grid), dim3(kTcThreads), smem, st, m[0], m[1], m[2], m[3], a);
+    if constexpr (PAIR) return launch_pdl_clusters(kern, dim3(grid), dim3(kTcThreads), smem, st, 2, m[0], m[1], tails, a);
+    return launch_pdl(kern, dim3(grid), dim3(kTcThreads), smem, st, m[0], m[1], tails, a);
 }
 
 // A pair's tiles of 256 features, or one CTA's of 128 where there are no more, or (forward, dx: 576 features 46 -> 36 us)
 // where those cover a tenth less that does not exist; a pair does the same work about a tenth faster.
 template <typename T, int MODE, int COLS, bool GATHER>
-cudaError_t run_shape(const CUtensorMap (&m)[4], const TcArgs& a, cudaStream_t st) {
+cudaError_t run_shape(const CUtensorMap (&m)[2], const Tails& tails, const TcArgs& a, cudaStream_t st) {
     if constexpr (COLS == 256) {
         const int whole = (a.feats + 255) / 256 * 256, half = (a.feats + 127) / 128 * 128;
-        if (MODE == kExpertDw ? a.feats > kFeat : whole * 10 <= half * 11) return run_tc<T, MODE, COLS, GATHER, true>(m, a, st);
+        if (MODE == kExpertDw ? a.feats > kFeat : whole * 10 <= half * 11) return run_tc<T, MODE, COLS, GATHER, true>(m, tails, a, st);
     }
-    return run_tc<T, MODE, COLS, GATHER, false>(m, a, st);
+    return run_tc<T, MODE, COLS, GATHER, false>(m, tails, a, st);
 }
 
 template <typename T>
 cudaError_t run_kind(const ExpertCall& c, const Operands& o, cudaStream_t st) {
-    CUtensorMap m[4];
+    CUtensorMap m[2];
+    Tails tails = {};
     TcArgs a = {};
     a.offsets = c.offsets;
     a.rows = o.rows;
@@ -631,12 +644,11 @@ cudaError_t run_kind(const ExpertCall& c, const Operands& o, cudaStream_t st) {
             a.out_vec = whole(c.y, c.n);
             a.ldo = c.n;
             ok = make_map(&m[0], c.dtype, o.w, c.d, c.n, c.experts, o.ldw, kFeat) &&
-                 make_map(&m[2], c.dtype, o.x, c.d, o.x_rows, 0, o.ldx, 32) &&
-                 make_map(&m[3], c.dtype, o.x, c.d, o.x_rows, 0, o.ldx, 1);
-            m[1] = m[0];
+                 make_map(&m[1], c.dtype, o.x, c.d, o.x_rows, 0, o.ldx, 32) &&
+                 make_map(&tails.b_row, c.dtype, o.x, c.d, o.x_rows, 0, o.ldx, 1);
             if (!ok) return cudaErrorInvalidValue;
-            if (few) return o.rows ? run_shape<T, kExpertForward, 64, true>(m, a, st) : run_shape<T, kExpertForward, 64, false>(m, a, st);
-            return run_shape<T, kExpertForward, 256, false>(m, a, st);
+            if (few) return o.rows ? run_shape<T, kExpertForward, 64, true>(m, tails, a, st) : run_shape<T, kExpertForward, 64, false>(m, tails, a, st);
+            return run_shape<T, kExpertForward, 256, false>(m, tails, a, st);
         case kExpertDx:
             a.rows = nullptr;
             a.x_rows = c.pairs;
@@ -646,11 +658,9 @@ cudaError_t run_kind(const ExpertCall& c, const Operands& o, cudaStream_t st) {
             a.out_vec = whole(c.dx, c.d);
             a.ldo = c.d;
             ok = make_map(&m[0], c.dtype, o.w, c.d, c.n, c.experts, o.ldw, kDepth) &&
-                 make_map(&m[2], c.dtype, o.dy, c.n, c.pairs, 0, o.lddy, 32);
-            m[1] = m[0];
-            m[3] = m[2];
+                 make_map(&m[1], c.dtype, o.dy, c.n, c.pairs, 0, o.lddy, 32);
             if (!ok) return cudaErrorInvalidValue;
-            return few ? run_shape<T, kExpertDx, 64, false>(m, a, st) : run_shape<T, kExpertDx, 256, false>(m, a, st);
+            return few ? run_shape<T, kExpertDx, 64, false>(m, tails, a, st) : run_shape<T, kExpertDx, 256, false>(m, tails, a, st);
         default:
             a.feats = c.n;
             a.cols = c.d;
@@ -658,11 +668,13 @@ cudaError_t run_kind(const ExpertCall& c, const Operands& o, cudaStream_t st) {
             a.out_vec = whole(c.dw, c.d);
             a.ldo = c.d;
             ok = make_map(&m[0], c.dtype, o.dy, c.n, c.pairs, 0, o.lddy, kDepth) &&
-                 make_map(&m[1], c.dtype, o.dy, c.n, c.pairs, 0, o.lddy, 1) &&
-                 make_map(&m[2], c.dtype, o.x, c.d, o.x_rows, 0, o.ldx, kDepth) &&
-                 make_map(&m[3], c.dtype, o.x, c.d, o.x_rows, 0, o.ldx, 1);
+                 make_map(&tails.a16, c.dtype, o.dy, c.n, c.pairs, 0, o.lddy, 16) &&
+                 make_map(&tails.a_row, c.dtype, o.dy, c.n, c.pairs, 0, o.lddy, 1) &&
+                 make_map(&m[1], c.dtype, o.x, c.d, o.x_rows, 0, o.ldx, kDepth) &&
+                 make_map(&tails.b16, c.dtype, o.x, c.d, o.x_rows, 0, o.ldx, 16) &&
+                 make_map(&tails.b_row, c.dtype, o.x, c.d, o.x_rows, 0, o.ldx, 1);
             if (!ok) return cudaErrorInvalidValue;
-            return run_shape<T, kExpertDw, 256, false>(m, a, st);
+            return run_shape<T, kExpertDw, 256, false>(m, tails, a, st);
     }
 }
 
