@@ -4,12 +4,13 @@
 // columns, a view that starts anywhere) is first copied to the workspace with its rows padded to 8 elements; the
 // padding is never read as data (the tensor maps end at the true column).
 //
-// Rows of x read by index: with few rows an expert the products' kernel gathers them itself (tile::gather4).  A gather
-// of four 128-byte pieces took 36 cycles of the TMA unit however it was issued, so a tile of 256 positions spent four
-// times as long on them as on its MMAs (8192 x 8 of 64 experts, 2048 x 2048: 2365 us, from grouped rows 529 us), and
-// warps that gather with 16-byte asynchronous copies took 1190 us (the hand-over of a stage from copies to tensor cores
-// takes longer than its MMAs).  With many rows an expert, and for dW, x is copied in grouped order first: 70 us there,
-// what writing it takes, of 560 in all.
+// Rows of x read by index: with up to 12 rows an expert on average the products' kernel gathers them itself
+// (tile::gather4).  A gather of four 128-byte pieces took 36 cycles of the TMA unit however it was issued, so a tile of
+// 256 positions spent four times as long on them as on its MMAs (8192 x 8 of 64 experts, 2048 x 2048: 2365 us, from
+// grouped rows 529 us), and warps that gather with 16-byte asynchronous copies took 1190 us (the hand-over of a stage
+// from copies to tensor cores takes longer than its MMAs).  With more rows an expert, and for dW, x is copied in grouped
+// order first: 70 us there, what writing it takes, of 560 in all (32 experts, 2048 x 2048: 6 rows each 57.4 us gathered,
+// 60.4 copied; 32 rows each 84.1 and 61.1).
 #include "common.cuh"
 #include "experts.cuh"
 #include "kmc_internal.h"
@@ -33,7 +34,9 @@ bool by_rows(const ExpertCall& c) {
     const int64_t used = c.pairs < c.experts ? c.pairs : c.experts;
     return c.pairs <= 4 * used || (c.pairs <= 16 * used && used * c.n * c.d <= (8 << 20));
 }
-bool takes_x(const ExpertCall& c) { return c.x && c.rows && !(c.kind == kExpertForward && expert_few_rows(c)); }
+bool takes_x(const ExpertCall& c) {
+    return c.x && c.rows && !(c.kind == kExpertForward && c.pairs <= 12 * (int64_t)c.experts);
+}
 
 // dst row i (cols elements, ldp apart) = src row idx[i], or row i without idx; zeros for a row outside src and in the
 // padding
@@ -108,9 +111,9 @@ struct Takes {
 
 }  // namespace
 
-// Positions per tile: 64 where the experts' mean is at most that (a stage is then 24 KB and eight are in flight), 256
-// above.
-bool expert_few_rows(const ExpertCall& c) { return c.pairs <= (int64_t)c.experts * 64; }
+// Positions per tile: 64 where the experts' mean is at most 40 (a stage is then 24 KB and eight are in flight), 256 above
+// (2048 x 2048, 32 experts: mean 32 61.4 us against 62.6, mean 64 73.8 against 65.3).
+bool expert_few_rows(const ExpertCall& c) { return c.pairs <= (int64_t)c.experts * 40; }
 
 size_t expert_bytes(const ExpertCall& c) {
     size_t need = 0;
