@@ -368,7 +368,8 @@ int kmc_group_rows(const int32_t *ids, int64_t rows, int choices, int experts, i
 
 /* y (pairs x n) = W_e x per position of expert e (offsets as kmc_group_rows gives them): x (x_rows x d, rows ldx apart),
  * W (experts x n x d).  group_row: the row of x each position reads (a row outside x reads zeros); NULL: x is already
- * grouped (x_rows = pairs).  Positions past offsets[experts] get zeros.  dtype KMC_BF16 or KMC_F16 throughout.
+ * grouped (x_rows = pairs).  Positions past offsets[experts] get zeros.  dtype KMC_BF16 or KMC_F16 throughout;
+ * pairs at most 2^31 - 1025, n and d at most 2^20.
  * kmc_expert_matmul_dx: dx (pairs x d) = W_e^T dy (pairs x n), by position (sum a row's positions with kmc_combine).
  * kmc_expert_matmul_dw: dW (experts x n x d) = sum over an expert's positions of dy x^T; 0 for an expert with none.
  * workspace: kmc_expert_bytes bytes for the call's operands (NULL for one it does not take), 256-byte aligned: room for

@@ -886,6 +886,9 @@ static int check_expert(const char* who, int64_t pairs, int experts, int n, int 
                         const void* error) {
     if (int s = check_dtype(who, dtype, false)) return s;
     if (int s = check_pairs(who, pairs, 1)) return s;
+    // the kernels count past a group's last position by up to a tile, in int32
+    if (pairs > INT32_MAX - 1024)
+        return fail(KMC_ERR_UNSUPPORTED, "%s: %lld positions, above 2^31 - 1025", who, (long long)pairs);
     if (int s = check_experts(who, experts)) return s;
     if (n < 1 || d < 1) return fail(KMC_ERR_INVALID, "%s: matrices of %d x %d", who, n, d);
     if (n > (1 << 20) || d > (1 << 20)) return fail(KMC_ERR_UNSUPPORTED, "%s: matrices of %d x %d, above 2^20", who, n, d);

@@ -37,6 +37,12 @@ __device__ __forceinline__ float unordered(unsigned u) {
 }
 __device__ __forceinline__ float sigmoid32(float l) { return __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-l))); }
 
+// exp of l - m <= 0 and the quotient of such by their sum (1 at least): the softmax's, by the hardware's exponential of
+// base 2.  Off by |x| 2^-23 + 2^-21 at most, relatively; below 2^-126 it is 0.  (The sigmoid, whose value decides a
+// choice bit for bit, takes expf and an IEEE division.)
+__device__ __forceinline__ float exp_below(float x) { return __expf(x); }
+__device__ __forceinline__ float share(float p, float total) { return __fdividef(p, total); }
+
 // Over the LANES lanes that share a row (aligned in the warp); every lane of the warp calls them.
 template <int LANES>
 __device__ __forceinline__ float row_sum(float v) {
@@ -278,7 +284,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
         m = row_max<LANES>(m);
         total = 0.0f;
 #pragma unroll
-        for (int i = 0; i < PER; i++) total += l[i] > -INFINITY ? expf(l[i] - m) : 0.0f;
+        for (int i = 0; i < PER; i++) total += l[i] > -INFINITY ? exp_below(l[i] - m) : 0.0f;
         total = row_sum<LANES>(total);
     }
     if constexpr (LANES == 32) {
@@ -299,9 +305,9 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
         }
     } else {
         if (a.renorm) m = row_max<LANES>(lm);
-        const float p = got ? expf(lm - m) : 0.0f;
+        const float p = got ? exp_below(lm - m) : 0.0f;
         if (a.renorm) total = row_sum<LANES>(p);
-        w = got ? p / total : 0.0f;
+        w = got ? share(p, total) : 0.0f;
     }
     if (here && lane < a.choices) {
         ids[t * a.choices + lane] = mine;
@@ -338,9 +344,9 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
         }
     } else if (a.renorm) {
         m = row_max<LANES>(lm);
-        p = got ? expf(lm - m) : 0.0f;
+        p = got ? exp_below(lm - m) : 0.0f;
         total = row_sum<LANES>(p);
-        p = got ? p / total : 0.0f;
+        p = got ? share(p, total) : 0.0f;
         dot = row_sum<LANES>(g * p);
     }
     float dl[PER];
@@ -355,11 +361,11 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
         total = 0.0f;
 #pragma unroll
         for (int i = 0; i < PER; i++) {
-            dl[i] = dl[i] > -INFINITY ? expf(dl[i] - m) : 0.0f;
+            dl[i] = dl[i] > -INFINITY ? exp_below(dl[i] - m) : 0.0f;
             total += dl[i];
         }
         total = row_sum<LANES>(total);
-        p = got ? expf(lm - m) / total : 0.0f;
+        p = got ? share(exp_below(lm - m), total) : 0.0f;
         dot = row_sum<LANES>(g * p);
         const float c = row_ballot<LANES>(got) != 0u ? -dot / total : 0.0f;   // a row with no choice: 0, whatever its logits
 #pragma unroll

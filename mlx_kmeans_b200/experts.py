@@ -12,6 +12,7 @@ All arguments are CUDA tensors; work is enqueued on the current stream and nothi
 expert_matmul and combine_rows are differentiable through torch.autograd; route_grad, expert_matmul_grad and
 combine_rows_grad are the same gradients as plain calls.  group_rows takes labels too (KMeans.labels_ on the device),
 to run one product per cluster.  Errors: ValueError for bad arguments, RuntimeError for a device failure.
+Calls can be captured in a CUDA graph, except a device's first expert_matmul (it allocates the word expert_status reads).
 """
 import os
 from typing import NamedTuple, Optional
@@ -56,7 +57,8 @@ def _tensors(*named):
 
 def expert_status(device=None):
     """Raise RuntimeError if an expert_matmul (or its gradient) on `device` gave up waiting on a barrier since the last
-    call, which leaves its result incomplete.  Waits for the device's current stream."""
+    call, which leaves its result incomplete: a fault of the library or the device, since no wait depends on the data.
+    Waits for the device's current stream."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     if _ext().status(device.index if device.index is not None else torch.cuda.current_device()):
         raise RuntimeError("expert_matmul: a kernel gave up waiting on a barrier; its result is incomplete")

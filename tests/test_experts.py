@@ -58,6 +58,7 @@ def test_expert_arguments():
 
     assert fwd(dtype=0) == bad and fwd(ldx=15) == bad and fwd(n=0) == bad and fwd(d=0) == bad and fwd(E=0) == bad
     assert fwd(pairs=-1) == bad and fwd(E=4097) == no and fwd(n=(1 << 20) + 1) == no and fwd(pairs=2 ** 31) == no
+    assert fwd(pairs=2 ** 31 - 1024) == no and b"positions" in L.kmc_last_error()
     assert fwd(w=None) == bad and fwd(off=None) == bad and fwd(err=None) == bad and fwd(y=None) == bad and fwd(x=None) == bad
     assert fwd(rows=None) == bad and b"grouped" in L.kmc_last_error()
     assert L.kmc_expert_matmul_dx(P, None, P, 8, 4, 8, 16, 1, P, None, 0, P, None) == bad
