@@ -340,7 +340,8 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
         dot = 0.0f;
         if (a.renorm) {
             total = row_sum<LANES>(s);
-            dot = total > 0.0f ? row_sum<LANES>(g * s) / total : 0.0f;
+            dot = row_sum<LANES>(g * s);                   // (by every row of the warp, those without a choice too)
+            dot = total > 0.0f ? dot / total : 0.0f;
         }
     } else if (a.renorm) {
         m = row_max<LANES>(lm);

@@ -178,6 +178,26 @@ def test_route_grad(case):
 
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("renorm", [False, True])
+@pytest.mark.parametrize("E,k", [(8, 2), (32, 8), (64, 8), (128, 16), (128, 20), (300, 4)])
+def test_route_rows_without_a_choice_beside_others(E, k, score, renorm):
+    """Rows that share a warp with masked rows, in every order: the weights and gradients of the rows alone."""
+    from mlx_kmeans_b200 import route, route_grad
+    T = 64
+    l = torch.randn(T, E, generator=rng(E), dtype=torch.float32).cuda()
+    mask = torch.rand(T, generator=rng(k)) < 0.5
+    g = torch.randn(T, k, generator=rng(1)).cuda()
+    ids, w = route(l, k, score=score, renormalize=renorm, mask=mask.cuda())
+    dl = route_grad(g, l, ids, score=score, renormalize=renorm)
+    alone_ids, alone_w = route(l[mask.cuda()], k, score=score, renormalize=renorm)
+    alone_dl = route_grad(g[mask.cuda()], l[mask.cuda()], alone_ids, score=score, renormalize=renorm)
+    assert torch.equal(ids[mask.cuda()], alone_ids) and torch.equal(w[mask.cuda()], alone_w)
+    assert torch.equal(dl[mask.cuda()], alone_dl)
+    off = ~mask.cuda()
+    assert int(ids[off].max()) == -1 and float(w[off].abs().max()) == 0.0 and float(dl[off].abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renorm", [False, True])
 def test_route_grad_against_differences(score, renorm):
     """The central difference of L = sum g w along a direction, the choice kept by logits 0.25 apart."""
     from mlx_kmeans_b200 import route
