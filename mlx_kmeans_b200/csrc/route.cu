@@ -75,15 +75,24 @@ __device__ __forceinline__ unsigned row_ballot(bool p) {   // bit i: lane i of t
     return (m >> (threadIdx.x & 31 & ~(LANES - 1))) & ((1u << (LANES & 31)) - 1u);
 }
 
-// The lane's PER logits of one row (-inf past the last expert).  vec: the row starts on a 16-byte boundary, or on
-// one of PER elements where that is less.
+// PER elements per lane as vectors of V (16 bytes, or all PER where that is less), or of half of that
 template <typename T, int PER>
-__device__ __forceinline__ void load_row(const T* row, int lane, int experts, bool vec, float (&l)[PER]) {
-    constexpr int V = PER * sizeof(T) >= 16 ? 16 / sizeof(T) : PER;
-    const int i0 = lane * PER;
+struct Vec {
+    static constexpr int V = PER * sizeof(T) >= 16 ? 16 / sizeof(T) : PER;
+    static constexpr int H = V > 1 ? V / 2 : 1;
+    static constexpr size_t BYTES = V * sizeof(T);
+    // 2: whole vectors are aligned, 1: halves of one, 0: elements only
+    static int level(const void* p, int64_t row_bytes) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(p) | (uintptr_t)row_bytes;
+        return at % BYTES == 0 ? 2 : at % (H * sizeof(T)) == 0 ? 1 : 0;
+    }
+};
+
+template <typename T, int PER, int V>
+__device__ __forceinline__ void load_by(const T* row, int i0, int experts, float (&l)[PER]) {
 #pragma unroll
     for (int i = 0; i < PER; i += V) {
-        if (vec && i0 + i + V <= experts) {
+        if (i0 + i + V <= experts) {
             const Pack<T, V> p = *reinterpret_cast<const Pack<T, V>*>(row + i0 + i);
 #pragma unroll
             for (int j = 0; j < V; j++) l[i + j] = Elem<T>::to(p.v[j]);
@@ -93,6 +102,36 @@ __device__ __forceinline__ void load_row(const T* row, int lane, int experts, bo
         }
     }
 }
+// The lane's PER logits of one row, -inf past the last expert
+template <typename T, int PER>
+__device__ __forceinline__ void load_row(const T* row, int lane, int experts, int level, float (&l)[PER]) {
+    if (level == 2) load_by<T, PER, Vec<T, PER>::V>(row, lane * PER, experts, l);
+    else if (level == 1) load_by<T, PER, Vec<T, PER>::H>(row, lane * PER, experts, l);
+    else load_by<T, PER, 1>(row, lane * PER, experts, l);
+}
+
+template <typename T, int PER, int V>
+__device__ __forceinline__ void store_by(T* row, int i0, int experts, const float (&l)[PER]) {
+#pragma unroll
+    for (int i = 0; i < PER; i += V) {
+        if (i0 + i + V <= experts) {
+            Pack<T, V> p;
+#pragma unroll
+            for (int j = 0; j < V; j++) p.v[j] = Elem<T>::from(l[i + j]);
+            *reinterpret_cast<Pack<T, V>*>(row + i0 + i) = p;
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; j++)
+                if (i0 + i + j < experts) row[i0 + i + j] = Elem<T>::from(l[i + j]);
+        }
+    }
+}
+template <typename T, int PER>
+__device__ __forceinline__ void store_row(T* row, int lane, int experts, int level, const float (&l)[PER]) {
+    if (level == 2) store_by<T, PER, Vec<T, PER>::V>(row, lane * PER, experts, l);
+    else if (level == 1) store_by<T, PER, Vec<T, PER>::H>(row, lane * PER, experts, l);
+    else store_by<T, PER, 1>(row, lane * PER, experts, l);
+}
 
 struct RouteArgs {
     int64_t rows, stride;
@@ -101,7 +140,7 @@ struct RouteArgs {
     const uint8_t* mask;
     float scale;
     int sigmoid, renorm;
-    int vec, out_vec;                                      // rows of logits / dlogits allow whole-vector accesses
+    int vec, out_vec;                                      // Vec::level of logits and dlogits
 };
 
 // Clears the keys of experts outside the best top_groups groups.  A group that covers a power of two of whole lanes
@@ -373,22 +412,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
         for (int i = 0; i < PER; i++) dl[i] = dl[i] != 0.0f ? c * dl[i] : 0.0f;
     }
     // the dense row first, then the chosen entries over it
-    constexpr int V = PER * sizeof(T) >= 16 ? 16 / sizeof(T) : PER;
-    const int i0 = lane * PER;
-#pragma unroll
-    for (int i = 0; i < PER; i += V) {
-        if (!here) {
-        } else if (a.out_vec && i0 + i + V <= a.experts) {
-            Pack<T, V> q;
-#pragma unroll
-            for (int j = 0; j < V; j++) q.v[j] = Elem<T>::from(dl[i + j]);
-            *reinterpret_cast<Pack<T, V>*>(out + i0 + i) = q;
-        } else {
-#pragma unroll
-            for (int j = 0; j < V; j++)
-                if (i0 + i + j < a.experts) out[i0 + i + j] = Elem<T>::from(dl[i + j]);
-        }
-    }
+    if (here) store_row<T, PER>(out, lane, a.experts, a.out_vec, dl);
     __syncwarp();
     if (here && got) {
         float v;
@@ -404,9 +428,8 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
 template <typename T, int LANES, int PER>
 cudaError_t run_route(const RouteCall& c, RouteArgs a, cudaStream_t st) {
     const int64_t rows = kRouteWarps * 32 / LANES, blocks = (a.rows + rows - 1) / rows;
-    const size_t step = PER * sizeof(T) >= 16 ? 16 : PER * sizeof(T);
-    a.vec = reinterpret_cast<uintptr_t>(c.logits) % step == 0 && (c.stride * sizeof(T)) % step == 0;
-    a.out_vec = reinterpret_cast<uintptr_t>(c.dlogits) % step == 0 && (c.experts * sizeof(T)) % step == 0;
+    a.vec = Vec<T, PER>::level(c.logits, c.stride * (int64_t)sizeof(T));
+    a.out_vec = Vec<T, PER>::level(c.dlogits, c.experts * (int64_t)sizeof(T));
     if (c.dweights == nullptr)
         return launch_pdl(k_route<T, LANES, PER>, dim3((unsigned)blocks), dim3(kRouteWarps * 32), 0, st,
                           static_cast<const T*>(c.logits), a, c.ids_out, c.weights);
@@ -429,11 +452,17 @@ cudaError_t run_route_type(const RouteCall& c, cudaStream_t st) {
     a.scale = c.scale;
     a.sigmoid = c.sigmoid;
     a.renorm = c.renorm;
-    // Eight or sixteen lanes a row where its experts fit and its choices do (lane j holds the j-th): the work that is
-    // done once a row is then shared by four or two rows.  Groups of experts are compared across a whole warp.
-    if (c.groups <= 1 && c.experts <= 64 && c.choices <= 8)
-        return c.experts <= 32 ? run_route<T, 8, 4>(c, a, st) : run_route<T, 8, 8>(c, a, st);
-    if (c.groups <= 1 && c.experts <= 128 && c.choices <= 16) return run_route<T, 16, 8>(c, a, st);
+    // Few lanes a row where its experts fit and its choices do (lane j holds the j-th): the work that is done once a row
+    // is then shared by several rows of a warp.  Groups of experts are compared across a whole warp.
+    if (c.groups <= 1) {
+        if (c.experts <= 64 && c.choices <= 4) return c.experts <= 32 ? run_route<T, 4, 8>(c, a, st) : run_route<T, 4, 16>(c, a, st);
+        if (c.experts <= 64 && c.choices <= 8) return c.experts <= 32 ? run_route<T, 8, 4>(c, a, st) : run_route<T, 8, 8>(c, a, st);
+        if (c.experts <= 128 && c.choices <= 8) return run_route<T, 8, 16>(c, a, st);
+        if (c.experts <= 128 && c.choices <= 16) return run_route<T, 16, 8>(c, a, st);
+        // (sixteen experts a lane take longer for one row: 160 experts, 100 rows 5.3 us at 32 lanes and 7.7 at 16,
+        // 8192 rows 13.7 and 12.9, 65536 rows 78.2 and 66.9)
+        if (c.experts <= 256 && c.choices <= 16 && c.rows >= 16384) return run_route<T, 16, 16>(c, a, st);
+    }
     if (c.experts <= 32) return run_route<T, 32, 1>(c, a, st);
     if (c.experts <= 64) return run_route<T, 32, 2>(c, a, st);
     if (c.experts <= 128) return run_route<T, 32, 4>(c, a, st);
