@@ -379,8 +379,9 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
         dot = 0.0f;
         if (a.renorm) {
             total = row_sum<LANES>(s);
-            dot = row_sum<LANES>(g * s);                   // (by every row of the warp, those without a choice too)
-            dot = total > 0.0f ? dot / total : 0.0f;
+            // (by every row of the warp, those without a choice too; the quotient first, so that a lone choice's share
+            // is 1 and its gradient 0)
+            dot = row_sum<LANES>(total > 0.0f ? g * (s / total) : 0.0f);
         }
     } else if (a.renorm) {
         m = row_max<LANES>(lm);

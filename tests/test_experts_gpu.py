@@ -197,6 +197,18 @@ def test_route_rows_without_a_choice_beside_others(E, k, score, renorm):
 
 
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E", [8, 64, 128, 256, 1000])
+def test_route_lone_renormalised_choice(E, score):
+    """One choice renormalised has the weight `scale` whatever its logit, and a gradient of exactly 0."""
+    from mlx_kmeans_b200 import route, route_grad
+    l = (torch.randn(300, E, generator=rng(E)) * 3).cuda()
+    ids, w = route(l, 1, score=score, scale=2.5)
+    assert torch.all(w == 2.5)
+    dl = route_grad(torch.randn(300, 1, generator=rng(1)).cuda(), l, ids, score=score, scale=2.5)
+    assert torch.all(dl == 0)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("renorm", [False, True])
 def test_route_grad_against_differences(score, renorm):
     """The central difference of L = sum g w along a direction, the choice kept by logits 0.25 apart."""
