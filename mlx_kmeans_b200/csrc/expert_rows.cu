@@ -11,6 +11,8 @@
 // WARPS = 1: a CTA is one warp over the whole depth.  WARPS = 4: four warps share the depth round by round and join
 // their float32 sums in shared memory, in a fixed order, the next block's first round under way meanwhile; taken where
 // there are too few blocks to go round (see run_rows).
+// One row of 8 of 64 experts, 2048 x 2048: 16.5 us for 67 MB (0.62 of the copy bandwidth: one round of loads, ramp and
+// tail count); 8 rows of them 62 us for 338 MB (0.83).
 // Any size, stride and alignment: 16-byte loads where every row starts on 16 bytes, element by element otherwise.
 #include <type_traits>
 
