@@ -624,16 +624,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
 // rows x dp bf16, row-major; box of `box_rows` rows x 64 columns, 128-byte swizzle, zero fill past the end
 bool make_map(CUtensorMap* m, const void* base, int64_t rows, int dp, int box_rows) {
-    auto fn = tensor_map_encode();
-    if (!fn) return false;
     cuuint64_t dims[2] = {(cuuint64_t)dp, (cuuint64_t)rows};
     cuuint64_t strides[1] = {(cuuint64_t)dp * 2};
     cuuint32_t box[2] = {(cuuint32_t)BK, (cuuint32_t)box_rows};
     cuuint32_t estr[2] = {1, 1};
-    CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
-                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS;
+    return encode_tensor_map(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
+                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
 template <int BN, bool AR, bool APPROX, bool CHUNK = false>

@@ -185,4 +185,20 @@ inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encode() {
     return fn;
 }
 
+// Encodes a tiled tensor map (the arguments of cuTensorMapEncodeTiled).  The driver's call wants a current context, which
+// a thread has only after its first call of the runtime that needs one: where it has none (a product's gradient as the
+// first work of the autograd engine's thread, say), the current device's primary context is made current.
+template <typename... Args>
+inline bool encode_tensor_map(CUtensorMap* m, Args... args) {
+    const auto fn = tensor_map_encode();
+    if (!fn) return false;
+    CUresult r = fn(m, args...);
+    if (r == CUDA_ERROR_INVALID_CONTEXT) {
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return false;
+        r = fn(m, args...);
+    }
+    return r == CUDA_SUCCESS;
+}
+
 }  // namespace kmc
