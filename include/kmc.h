@@ -370,7 +370,11 @@ int kmc_group_rows(const int32_t *ids, int64_t rows, int choices, int experts, i
  * W (experts x n x d).  group_row: the row of x each position reads (a row outside x reads zeros); NULL: x is already
  * grouped (x_rows = pairs).  Positions past offsets[experts] get zeros.  dtype KMC_BF16 or KMC_F16 throughout;
  * pairs at most 2^31 - 1025, n and d at most 2^20.
- * kmc_expert_matmul_dx: dx (pairs x d) = W_e^T dy (pairs x n), by position (sum a row's positions with kmc_combine).
+ * kmc_expert_matmul_dx: dx (pairs x d) = W_e^T dy (pairs x n), by position (x that was grouped).
+ * kmc_expert_matmul_dx_rows: dx (rows x d) of rows that were gathered: a row's positions (slot, rows x choices; pairs =
+ * rows * choices; a slot of -1 adds nothing) summed in float32 and rounded once.  Its workspace is
+ * kmc_expert_dx_rows_bytes, 256-byte aligned: the positions' gradients, float32 with more than one choice a row, and
+ * what kmc_expert_bytes gives for kmc_expert_matmul_dx.
  * kmc_expert_matmul_dw: dW (experts x n x d) = sum over an expert's positions of dy x^T; 0 for an expert with none.
  * workspace: kmc_expert_bytes bytes for the call's operands (NULL for one it does not take), 256-byte aligned: room for
  * x in grouped order where that is read faster, and for padded copies of operands that do not start on 16 bytes or have
@@ -383,6 +387,10 @@ int kmc_expert_matmul(const void *x, int64_t x_rows, int64_t ldx, const int32_t 
                       void *workspace, size_t ws_bytes, int32_t *error, void *stream);
 int kmc_expert_matmul_dx(const void *dy, const void *w, const int32_t *offsets, int64_t pairs, int experts, int n,
                          int d, int dtype, void *dx, void *workspace, size_t ws_bytes, int32_t *error, void *stream);
+size_t kmc_expert_dx_rows_bytes(const void *w, const void *dy, int64_t rows, int choices, int experts, int n, int d);
+int kmc_expert_matmul_dx_rows(const void *dy, const void *w, const int32_t *offsets, const int32_t *slot, int64_t rows,
+                              int choices, int experts, int n, int d, int dtype, void *dx, void *workspace,
+                              size_t ws_bytes, int32_t *error, void *stream);
 int kmc_expert_matmul_dw(const void *dy, const void *x, int64_t x_rows, int64_t ldx, const int32_t *group_row,
                          const int32_t *offsets, int64_t pairs, int experts, int n, int d, int dtype, void *dw,
                          void *workspace, size_t ws_bytes, int32_t *error, void *stream);

@@ -85,6 +85,8 @@ SIGNATURES = {
     "kmc_expert_matmul": (_int, [_vp, _i64, _i64, _vp, _vp, _vp, _i64, _int, _int, _int, _int, _vp, _vp, _sz, _vp,
                                  _vp]),
     "kmc_expert_matmul_dx": (_int, [_vp, _vp, _vp, _i64, _int, _int, _int, _int, _vp, _vp, _sz, _vp, _vp]),
+    "kmc_expert_dx_rows_bytes": (_sz, [_vp, _vp, _i64, _int, _int, _int, _int]),
+    "kmc_expert_matmul_dx_rows": (_int, [_vp, _vp, _vp, _vp, _i64, _int, _int, _int, _int, _int, _vp, _vp, _sz, _vp, _vp]),
     "kmc_expert_matmul_dw": (_int, [_vp, _vp, _i64, _i64, _vp, _vp, _i64, _int, _int, _int, _int, _vp, _vp, _sz, _vp,
                                     _vp]),
     "kmc_combine": (_int, [_vp, _int, _i64, _int, _int, _vp, _vp, _vp, _vp]),

@@ -882,6 +882,17 @@ int kmc_group_rows(const int32_t* ids, int64_t rows, int choices, int experts, i
     return KMC_OK;
 }
 
+static int check_combine(const char* who, int dtype, int64_t rows, int choices, int width) {
+    if (int s = check_dtype(who, dtype, true)) return s;
+    if (int s = check_pairs(who, rows, choices)) return s;
+    if (width < 1) return fail(KMC_ERR_INVALID, "%s: width must be >= 1, got %d", who, width);
+    if (width > (1 << 20)) return fail(KMC_ERR_UNSUPPORTED, "%s: width %d, above 2^20", who, width);
+    // one block per 256 elements at the least favourable alignment: the grid's limit of 2^31 - 1 blocks
+    if (rows * (int64_t)width / 256 >= INT32_MAX)
+        return fail(KMC_ERR_UNSUPPORTED, "%s: %lld rows of %d features", who, (long long)rows, width);
+    return KMC_OK;
+}
+
 static int check_expert(const char* who, int64_t pairs, int experts, int n, int d, int dtype, const void* offsets,
                         const void* error) {
     if (int s = check_dtype(who, dtype, false)) return s;
@@ -955,6 +966,64 @@ int kmc_expert_matmul_dx(const void* dy, const void* w, const int32_t* offsets, 
     return run_expert("kmc_expert_matmul_dx", c, ws_bytes, stream);
 }
 
+// The gradients by position, in front of the product's own workspace: float32 where several are summed; 16-bit for one
+// choice a row, which is rounded once as it is
+static size_t dx_positions_bytes(int64_t pairs, int choices, int d) {
+    return ((size_t)pairs * d * (choices > 1 ? 4 : 2) + 255) & ~size_t(255);
+}
+
+static ExpertCall dx_call(const void* dy, const void* w, int64_t pairs, int experts, int n, int d) {
+    ExpertCall c = {};
+    c.kind = kExpertDx;
+    c.dy = dy;
+    c.w = w;
+    c.pairs = pairs;
+    c.experts = experts;
+    c.n = n;
+    c.d = d;
+    return c;
+}
+
+size_t kmc_expert_dx_rows_bytes(const void* w, const void* dy, int64_t rows, int choices, int experts, int n, int d) {
+    if (rows < 0 || choices < 1 || rows > INT32_MAX / choices || experts < 1 || n < 1 || d < 1) return 0;
+    return dx_positions_bytes(rows * choices, choices, d) + expert_bytes(dx_call(dy, w, rows * choices, experts, n, d));
+}
+
+int kmc_expert_matmul_dx_rows(const void* dy, const void* w, const int32_t* offsets, const int32_t* slot, int64_t rows,
+                              int choices, int experts, int n, int d, int dtype, void* dx, void* workspace,
+                              size_t ws_bytes, int32_t* error, void* stream) {
+    const char* who = "kmc_expert_matmul_dx_rows";
+    if (int s = check_pairs(who, rows, choices)) return s;
+    if (int s = check_expert(who, rows * choices, experts, n, d, dtype, offsets, error)) return s;
+    if (int s = check_combine(who, dtype, rows, choices, d)) return s;
+    if (!w || (rows > 0 && (!dy || !slot || !dx))) return fail(KMC_ERR_INVALID, "%s: null pointer", who);
+    if (rows == 0) return KMC_OK;
+    const size_t need = kmc_expert_dx_rows_bytes(w, dy, rows, choices, experts, n, d);
+    if (!workspace || ws_bytes < need)
+        return fail(KMC_ERR_INVALID, "%s: workspace of %zu bytes, need %zu", who, workspace ? ws_bytes : (size_t)0, need);
+    const size_t front = dx_positions_bytes(rows * choices, choices, d);
+    ExpertCall c = dx_call(dy, w, rows * choices, experts, n, d);
+    c.dtype = dtype;
+    c.offsets = offsets;
+    c.dx = workspace;
+    c.dx_f32 = choices > 1;
+    c.ws = static_cast<char*>(workspace) + front;
+    c.error = error;
+    if (int s = run_expert(who, c, ws_bytes - front, stream)) return s;
+    CombineCall m = {};
+    m.y = workspace;
+    m.slot = slot;
+    m.tokens = rows;
+    m.choices = choices;
+    m.width = d;
+    m.dtype = dtype;
+    m.sum_f32 = choices > 1;
+    m.out = dx;
+    cudaError_t e = launch_combine(m, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, who);
+    return KMC_OK;
+}
+
 int kmc_expert_matmul_dw(const void* dy, const void* x, int64_t x_rows, int64_t ldx, const int32_t* group_row,
                          const int32_t* offsets, int64_t pairs, int experts, int n, int d, int dtype, void* dw,
                          void* workspace, size_t ws_bytes, int32_t* error, void* stream) {
@@ -999,17 +1068,6 @@ size_t kmc_expert_bytes(const void* x, int64_t x_rows, int64_t ldx, const int32_
     c.n = n;
     c.d = d;
     return expert_bytes(c);
-}
-
-static int check_combine(const char* who, int dtype, int64_t rows, int choices, int width) {
-    if (int s = check_dtype(who, dtype, true)) return s;
-    if (int s = check_pairs(who, rows, choices)) return s;
-    if (width < 1) return fail(KMC_ERR_INVALID, "%s: width must be >= 1, got %d", who, width);
-    if (width > (1 << 20)) return fail(KMC_ERR_UNSUPPORTED, "%s: width %d, above 2^20", who, width);
-    // one block per 256 elements at the least favourable alignment: the grid's limit of 2^31 - 1 blocks
-    if (rows * (int64_t)width / 256 >= INT32_MAX)
-        return fail(KMC_ERR_UNSUPPORTED, "%s: %lld rows of %d features", who, (long long)rows, width);
-    return KMC_OK;
 }
 
 int kmc_combine(const void* y, int dtype, int64_t rows, int choices, int width, const int32_t* slot,

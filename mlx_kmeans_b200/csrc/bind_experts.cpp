@@ -309,15 +309,23 @@ Tensor expert_dx(const Tensor& dy0, const Tensor& w0, const Tensor& offsets, con
     const c10::cuda::CUDAGuard guard(w0.device());
     const Tensor dy = dy0.contiguous(), w = w0.contiguous();
     const int E = as_int(g.E, "n_experts"), N = as_int(w.size(1), "n"), D = as_int(w.size(2), "d");
+    if (gather) {
+        const int k = as_int(g.k, "choices");
+        const size_t need = kmc_expert_dx_rows_bytes(data(w), data(dy), g.T, k, E, N, D);
+        const Tensor ws = workspace(need, w);
+        Tensor dx = empty({g.T, D}, w.scalar_type(), w);
+        check(kmc_expert_matmul_dx_rows(data(dy), data(w), g.off(), ptr<int32_t>(slot), g.T, k, E, N, D, type, data(dx),
+                                        need ? data(ws) : nullptr, need, error_word(w), stream(w)),
+              "kmc_expert_matmul_dx_rows");
+        return dx;
+    }
     const size_t need = kmc_expert_bytes(nullptr, 0, D, nullptr, data(w), data(dy), g.P, E, N, D);
     const Tensor ws = workspace(need, w);
     Tensor dx = empty({g.P, D}, w.scalar_type(), w);
     check(kmc_expert_matmul_dx(data(dy), data(w), g.off(), g.P, E, N, D, type, data(dx), need ? data(ws) : nullptr, need,
                                error_word(w), stream(w)),
           "kmc_expert_matmul_dx");
-    // a row with several choices: the float32 sum of its positions' gradients, which are in w's type by now (each
-    // rounded once; the error of the sum stays within that of one more rounding of its result)
-    return gather ? combine_of(dx, type, g, {}) : dx;
+    return dx;
 }
 
 Tensor expert_dw(const Tensor& dy0, const Tensor& x0, const Tensor& offsets, const Tensor& rows, const Tensor& slot,

@@ -2,12 +2,15 @@
 //
 //   out_t = sum_j w_tj y_slot(t,j)          dy_slot(t,j) = w_tj dout_t          dw_tj = <dout_t, y_slot(t,j)>
 // w = 1 without weights; a pair with slot -1 adds nothing (dw 0), and a row of dy that no pair has is 0.  Sums run in
-// float32 in the order j = 0 .. k - 1 (out) or in a fixed tree over the row (dw), and are rounded once when stored.
+// float32 in the order j = 0 .. k - 1 (out) or in a fixed tree over the row (dw), and are rounded once when stored; y may
+// be float32 where out is 16-bit (a row's gradients by position, from expert_tc.cu).
 //
 // Memory bound.  Forward: one thread per 16 bytes of out, its k reads of y independent and in flight together; each
 // row of y is read once and each row of out written once.  Backward: one warp per pair reads dout_t (the k warps of a
 // row run side by side, so it comes from L1 / L2 after the first) and y's row once and writes dy's row.  16384 rows of 8
 // choices, 2048 features, bfloat16: both in 277 us, where their bytes (1.74 GB) take 266 at the copy bandwidth.
+#include <type_traits>
+
 #include "common.cuh"
 #include "experts.cuh"
 #include "kmc_internal.h"
@@ -26,8 +29,8 @@ struct CombineArgs {
     int choices, width;                   // width: features
 };
 
-template <typename T, int V>
-__global__ void __launch_bounds__(kCombineThreads) k_combine(const T* __restrict__ y, CombineArgs a, T* __restrict__ out) {
+template <typename T, typename O, int V>
+__global__ void __launch_bounds__(kCombineThreads) k_combine(const T* __restrict__ y, CombineArgs a, O* __restrict__ out) {
     pdl_wait();
     const int vecs = a.width / V;
     const int64_t i = (int64_t)blockIdx.x * kCombineThreads + threadIdx.x;
@@ -47,10 +50,10 @@ __global__ void __launch_bounds__(kCombineThreads) k_combine(const T* __restrict
 #pragma unroll
         for (int v = 0; v < V; v++) acc[v] = fmaf(w, Elem<T>::to(p.v[v]), acc[v]);
     }
-    Pack<T, V> r;
+    Pack<O, V> r;
 #pragma unroll
-    for (int v = 0; v < V; v++) r.v[v] = Elem<T>::from(acc[v]);
-    *reinterpret_cast<Pack<T, V>*>(out + t * a.width + f) = r;
+    for (int v = 0; v < V; v++) r.v[v] = Elem<O>::from(acc[v]);
+    *reinterpret_cast<Pack<O, V>*>(out + t * a.width + f) = r;
 }
 
 template <typename T, int V>
@@ -96,7 +99,7 @@ __global__ void __launch_bounds__(kCombineThreads)
     }
 }
 
-template <typename T, int V>
+template <typename T, typename O, int V>
 cudaError_t run_combine(const CombineCall& c, cudaStream_t st) {
     CombineArgs a;
     a.slot = c.slot;
@@ -108,32 +111,36 @@ cudaError_t run_combine(const CombineCall& c, cudaStream_t st) {
     a.width = c.width;
     if (c.dout == nullptr) {
         const int64_t blocks = (a.tokens * (a.width / V) + kCombineThreads - 1) / kCombineThreads;
-        return launch_pdl(k_combine<T, V>, dim3((unsigned)blocks), dim3(kCombineThreads), 0, st,
-                          static_cast<const T*>(c.y), a, static_cast<T*>(c.out));
+        return launch_pdl(k_combine<T, O, V>, dim3((unsigned)blocks), dim3(kCombineThreads), 0, st,
+                          static_cast<const T*>(c.y), a, static_cast<O*>(c.out));
     }
-    const int64_t blocks = (a.pairs + kCombineThreads / 32 - 1) / (kCombineThreads / 32);
-    return launch_pdl(k_combine_grad<T, V>, dim3((unsigned)blocks), dim3(kCombineThreads), 0, st,
-                      static_cast<const T*>(c.dout), static_cast<const T*>(c.y), a, static_cast<T*>(c.dy),
-                      c.dweights);
+    if constexpr (std::is_same<T, O>::value) {
+        const int64_t blocks = (a.pairs + kCombineThreads / 32 - 1) / (kCombineThreads / 32);
+        return launch_pdl(k_combine_grad<T, V>, dim3((unsigned)blocks), dim3(kCombineThreads), 0, st,
+                          static_cast<const T*>(c.dout), static_cast<const T*>(c.y), a, static_cast<T*>(c.dy),
+                          c.dweights);
+    }
+    return cudaErrorInvalidValue;         // (no gradient of the form with a float32 y)
 }
 
-// 16 bytes per access where every row starts on a 16-byte boundary, one element otherwise
-template <typename T>
+// 16 bytes per access to y where every row starts on a 16-byte boundary, one element otherwise
+template <typename T, typename O>
 cudaError_t run_combine_type(const CombineCall& c, cudaStream_t st) {
     constexpr int V = 16 / sizeof(T);
     auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
     if (c.width % V == 0 && aligned(c.y) && aligned(c.out) && aligned(c.dout) && aligned(c.dy))
-        return run_combine<T, V>(c, st);
-    return run_combine<T, 1>(c, st);
+        return run_combine<T, O, V>(c, st);
+    return run_combine<T, O, 1>(c, st);
 }
 
 }  // namespace
 
 cudaError_t launch_combine(const CombineCall& c, cudaStream_t st) {
     switch (c.dtype) {
-        case 0: return run_combine_type<float>(c, st);
-        case 1: return run_combine_type<__nv_bfloat16>(c, st);
-        default: return run_combine_type<__half>(c, st);
+        case 0: return run_combine_type<float, float>(c, st);
+        case 1:
+            return c.sum_f32 ? run_combine_type<float, __nv_bfloat16>(c, st) : run_combine_type<__nv_bfloat16, __nv_bfloat16>(c, st);
+        default: return c.sum_f32 ? run_combine_type<float, __half>(c, st) : run_combine_type<__half, __half>(c, st);
     }
 }
 

@@ -3,7 +3,8 @@
 //   forward  y_p  = W_e x_row(p)              positions p of expert e: offsets[e] <= p < offsets[e + 1]
 //   dx       dx_p = W_e^T dy_p
 //   dW       dW_e = sum_p dy_p x_row(p)^T
-// 16-bit operands, float32 accumulation in TMEM, one rounding to 16 bits when a result is stored.
+// 16-bit operands, float32 accumulation in TMEM, one rounding to 16 bits when a result is stored; dx can be stored in
+// float32, for rows whose positions are summed afterwards.
 //
 // The matrix is the MMA's A operand: features are its M rows, and up to COLS positions its N columns.  N is a run-time
 // field of the instruction, so a group of any number of rows costs that number rounded up to 16 (32 for a pair of
@@ -59,6 +60,7 @@ struct TcArgs {
     int most;                             // positions per tile at most (forward, dx): COLS, or fewer (see run_tc)
     void* out;
     int64_t ldo;                          // row length of out
+    int out_f32;                          // dx: out is float32
     int out_vec;                          // rows of out start on 16-byte boundaries
     int* error;
 };
@@ -223,6 +225,33 @@ __device__ __forceinline__ void store_positions(T* dst, int64_t ldo, int left, i
 #pragma unroll
         for (int j = 0; j < 32; j++)
             if (j < left) dst[(int64_t)j * ldo + lane] = Elem<T>::from(v[j]);
+    }
+}
+
+// The same in float32, 16 columns at a time: 128-byte runs.
+__device__ __forceinline__ void store_positions_f32(float* dst, int64_t ldo, int left, int feats, bool vec,
+                                                    const float (&v)[32], unsigned char* stash) {
+    const int lane = threadIdx.x & 31;
+    if (vec) {
+        float* w = reinterpret_cast<float*>(stash);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+#pragma unroll
+            for (int j = 0; j < 16; j++) w[j * 36 + lane] = v[16 * h + j];
+            __syncwarp();
+            const int g = (lane & 7) * 4;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int j = (lane >> 3) + 4 * i;
+                if (g < feats && 16 * h + j < left)        // feats is a multiple of 4 here
+                    *reinterpret_cast<float4*>(dst + (int64_t)(16 * h + j) * ldo + g) = *reinterpret_cast<const float4*>(w + j * 36 + g);
+            }
+            __syncwarp();
+        }
+    } else if (lane < feats) {
+#pragma unroll
+        for (int j = 0; j < 32; j++)
+            if (j < left) dst[(int64_t)j * ldo + lane] = v[j];
     }
 }
 
@@ -516,14 +545,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int q = warp & 3;
         const uint32_t lane_base = tmem + ((uint32_t)(32 * q) << 16);
         T* out = static_cast<T*>(a.out);
+        float* out32 = static_cast<float*>(a.out);
+        const bool f32 = MODE == kExpertDx && a.out_f32;
         unsigned char* mine = stash + q * kEpiBytes;
         uint32_t abuf = 0, aphase = 0;
         bool ok = true;
         if constexpr (MODE != kExpertDw) {                 // rows past the last group: zeros
             const int64_t taken = min(max(__ldg(a.offsets + a.experts), 0), a.pairs);
             for (int64_t i = taken * a.ldo + (int64_t)blockIdx.x * kEpiThreads + threadIdx.x - 64;
-                 i < a.pairs * a.ldo; i += (int64_t)gridDim.x * kEpiThreads)
-                out[i] = Elem<T>::from(0.0f);
+                 i < a.pairs * a.ldo; i += (int64_t)gridDim.x * kEpiThreads) {
+                if (f32) out32[i] = 0.0f;
+                else out[i] = Elem<T>::from(0.0f);
+            }
         }
         for (int64_t t = t0; t < tiles && ok; t += dt) {
             const Tile w = Sh::at(a, first, t, e);
@@ -544,6 +577,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if constexpr (MODE == kExpertDw)
                     store_features<T>(out + ((int64_t)w.e * a.feats + f) * a.ldo + w.c0 + c, a.ldo, a.cols - w.c0 - c,
                                       a.feats - f, a.out_vec, v, mine);
+                else if (f32)
+                    store_positions_f32(out32 + (int64_t)(w.p0 + c) * a.ldo + f, a.ldo, w.p1 - w.p0 - c, a.feats - f, a.out_vec,
+                                        v, mine);
                 else
                     store_positions<T>(out + (int64_t)(w.p0 + c) * a.ldo + f, a.ldo, w.p1 - w.p0 - c, a.feats - f, a.out_vec,
                                        v, mine);
@@ -657,7 +693,8 @@ cudaError_t run_kind(const ExpertCall& c, const Operands& o, cudaStream_t st) {
             a.feats = c.d;
             a.depth = c.n;
             a.out = c.dx;
-            a.out_vec = whole(c.dx, c.d);
+            a.out_f32 = c.dx_f32;
+            a.out_vec = c.dx_f32 ? c.d % 4 == 0 && reinterpret_cast<uintptr_t>(c.dx) % 16 == 0 : whole(c.dx, c.d);
             a.ldo = c.d;
             ok = make_map(&m[0], c.dtype, o.w, c.d, c.n, c.experts, o.ldw, kDepth) &&
                  make_map(&m[1], c.dtype, o.dy, c.n, c.pairs, 0, o.lddy, 32);

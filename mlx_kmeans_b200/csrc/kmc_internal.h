@@ -259,11 +259,12 @@ cudaError_t launch_group(const int32_t* ids, int64_t pairs, int choices, int exp
                          int32_t* slot, void* ws, cudaStream_t st);
 
 struct CombineCall {
-    const void* y;            // pairs x width
+    const void* y;            // pairs x width, float32 where sum_f32 is set, of dtype otherwise
     const int32_t* slot;      // tokens x choices
     const float* weights;     // tokens x choices, or nullptr: 1
     int64_t tokens;
     int choices, width, dtype;
+    int sum_f32;              // forward, dtype 16-bit: y is float32 and rounded in out for the first time
     void* out;                // forward: tokens x width
     const void* dout;         // gradient (nullptr: forward)
     const int32_t* taken;     // device: positions with a pair
@@ -285,6 +286,7 @@ struct ExpertCall {
     int64_t pairs;
     int experts, n, d;
     void *y, *dx, *dw;        // the output of each kind
+    int dx_f32;               // dx is float32
     void* ws;                 // expert_bytes(call) bytes
     int* error;               // set to 1 by a kernel that gave up on a barrier
 };

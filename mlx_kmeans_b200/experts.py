@@ -159,7 +159,7 @@ def expert_matmul(x, w, groups, *, gather=True):
 
 def expert_matmul_grad(dy, x, w, groups, *, gather=True):
     """The gradients of expert_matmul for dy (positions, n): dx in x's shape (with gather=True a row's positions are
-    summed) and dw in w's; an expert with no position gets a dw of zeros."""
+    summed in float32 and the sum is rounded) and dw in w's; an expert with no position gets a dw of zeros."""
     _tensors((dy, "dy"), (x, "x"), (w, "w"))
     if x.ndim == 2 and w.ndim == 3 and x.shape[1] != w.shape[2]:
         raise ValueError(f"x has {x.shape[1]} columns, the matrices {w.shape[2]}")

@@ -1,0 +1,23 @@
+"""Routed experts: argument checks of the C entry points and Python functions beyond test_experts.py (no GPU: every call
+below is refused before any CUDA call)."""
+from test_experts import P, lib
+
+
+def test_dx_rows_arguments():
+    _l, L = lib()
+    bad, no = _l.KMC_ERR_INVALID, _l.KMC_ERR_UNSUPPORTED
+
+    def call(dy=P, w=P, off=P, slot=P, rows=4, choices=2, E=4, n=8, d=16, dtype=1, dx=P, ws=P, nb=1 << 20, err=P):
+        return L.kmc_expert_matmul_dx_rows(dy, w, off, slot, rows, choices, E, n, d, dtype, dx, ws, nb, err, None)
+
+    assert call(rows=-1) == bad and call(choices=0) == bad and call(E=0) == bad and call(n=0) == bad and call(d=0) == bad
+    assert call(dtype=0) == bad and call(dtype=3) == bad
+    assert call(rows=2 ** 30, choices=2) == no and call(E=4097) == no and call(d=(1 << 20) + 1) == no
+    for missing in ("dy", "w", "off", "slot", "dx", "err"):
+        assert call(**{missing: None}) == bad and b"null" in L.kmc_last_error()
+    need = L.kmc_expert_dx_rows_bytes(P, P, 4, 2, 4, 8, 16)
+    assert need == 4 * 2 * 16 * 4 and call(nb=need - 1) == bad and b"workspace" in L.kmc_last_error()
+    assert call(ws=None) == bad
+    assert L.kmc_expert_dx_rows_bytes(P, P, 4, 1, 4, 8, 16) == 256                  # 16-bit: nothing is summed
+    assert L.kmc_expert_dx_rows_bytes(P, P, 4, 2, 4, 8, 15) == 512 + 4 * 8 * 16 * 2  # and W's rows padded
+    assert call(rows=0, dy=None, slot=None, dx=None, ws=None, nb=0) == _l.KMC_OK

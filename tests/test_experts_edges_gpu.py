@@ -88,3 +88,61 @@ def test_first_backward_of_the_autograd_thread():
     """
     r = subprocess.run([sys.executable, "-c", textwrap.dedent(code)], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "backward" in r.stdout, r.stderr
+
+
+# ---------------------------------------------------------------- the gradient of gathered rows
+
+def by_row(groups, v):
+    """float64 values by position summed over each row's pairs."""
+    slot = groups.slot.cpu().long()
+    slot = slot if slot.ndim == 2 else slot[:, None]
+    return torch.where((slot >= 0)[:, :, None], v[slot.clamp(min=0)], 0.0).sum(1)
+
+
+@pytest.mark.parametrize("dt", HALF)
+@pytest.mark.parametrize("shape", [(1, 4, 8, 40, 64), (5, 2, 4, 129, 264), (48, 4, 12, 200, 336), (64, 2, 5, 33, 35),
+                                   (333, 3, 5, 77, 51), (700, 3, 7, 384, 192), (1100, 2, 3, 136, 1002), (300, 8, 16, 64, 4),
+                                   (900, 2, 2, 130, 577)])
+def test_dx_of_a_row_is_rounded_once(shape, dt):
+    """A row's positions are summed in float32, and only the sum is rounded: no term's own rounding enters."""
+    from mlx_kmeans_b200 import expert_matmul_grad
+    T, k, E, N, D = shape
+    g = rng(T + D)
+    groups = plan(T, k, E, T)
+    x = torch.randn(T, D, generator=g).to(dt).cuda()
+    w = (torch.randn(E, N, D, generator=g) / N ** 0.5).to(dt).cuda()
+    dy = torch.randn(T * k, N, generator=g).to(dt).cuda()
+    dx, _ = expert_matmul_grad(dy, x, w, groups)
+    _, (rx, xm), _ = ref_matmul(x, w, groups, True, dy)
+    assert dx.dtype == dt
+    near(dx, by_row(groups, rx), by_row(groups, xm), N + k)
+
+
+@pytest.mark.parametrize("dt", HALF)
+@pytest.mark.parametrize("T,D", [(1, 16), (5, 33), (700, 264), (200, 2)])
+def test_dx_terms_past_the_types_range_cancel(T, D, dt):
+    """Two positions of a row with gradients of +70000 and -70000, which float16 does not hold: their sum is 0."""
+    from mlx_kmeans_b200 import expert_matmul, expert_matmul_grad, group_rows
+    groups = group_rows(torch.tensor([[0, 1]], dtype=torch.int32).repeat(T, 1).cuda(), 2)
+    w = torch.full((2, 8, D), 100.0)
+    w[1] = -100.0
+    w, x = w.to(dt).cuda(), torch.zeros(T, D, dtype=dt, device="cuda", requires_grad=True)
+    dy = torch.full((2 * T, 8), 87.5, dtype=dt, device="cuda")            # 8 * 87.5 * 100 = 70000
+    assert torch.equal(expert_matmul_grad(dy, x.detach(), w, groups)[0], torch.zeros_like(x))
+    expert_matmul(x, w, groups).backward(dy)
+    assert torch.equal(x.grad, torch.zeros_like(x))
+
+
+def test_dx_of_labels_and_of_single_choices():
+    """One choice a row: the position's gradient itself, 0 where the row has none."""
+    from mlx_kmeans_b200 import expert_matmul_grad, group_rows
+    for lab in (torch.randint(-1, 5, (300,), generator=rng(1), dtype=torch.int32),
+                torch.randint(-1, 5, (300, 1), generator=rng(2), dtype=torch.int32)):
+        groups = group_rows(lab.cuda(), 5)
+        g = rng(3)
+        x, w = torch.randn(300, 72, generator=g).half().cuda(), torch.randn(5, 40, 72, generator=g).half().cuda()
+        dy = torch.randn(300, 40, generator=g).half().cuda()
+        dx, _ = expert_matmul_grad(dy, x, w, groups)
+        _, (rx, xm), _ = ref_matmul(x, w, groups, True, dy)
+        near(dx, by_row(groups, rx), by_row(groups, xm), 40)
+        assert int(dx[lab.reshape(-1).cuda() < 0].abs().max()) == 0
