@@ -398,12 +398,19 @@ int kmc_expert_matmul_dw(const void *dy, const void *x, int64_t x_rows, int64_t 
 /* out (rows x width) = sum over a row's choices of weight * y[slot] (y: rows * choices x width of `dtype`, by
  * position; weights: rows x choices float32, NULL: 1; a slot of -1 adds nothing).  kmc_combine_grad: dy (by position;
  * zeros from position *taken on, taken = offsets + experts of the plan, device) = weight * dout, and dweights (rows x
- * choices float32, NULL to skip) = <dout, y[slot]>, 0 for a slot of -1. */
+ * choices float32, NULL to skip) = <dout, y[slot]>, 0 for a slot of -1.  It wants a pair for every position below *taken,
+ * as kmc_group_rows leaves them, and does not write a row of dy without one.  kmc_combine_grad_slots: the same for slots
+ * of which any were set to -1 since (experts over their capacity): every row of dy that no slot names is zeros.
+ * workspace: kmc_combine_bytes(rows, choices) bytes, 4-byte aligned. */
 int kmc_combine(const void *y, int dtype, int64_t rows, int choices, int width, const int32_t *slot,
                 const float *weights, void *out, void *stream);
 int kmc_combine_grad(const void *dout, const void *y, int dtype, int64_t rows, int choices, int width,
                      const int32_t *slot, const float *weights, const int32_t *taken, void *dy, float *dweights,
                      void *stream);
+size_t kmc_combine_bytes(int64_t rows, int choices);
+int kmc_combine_grad_slots(const void *dout, const void *y, int dtype, int64_t rows, int choices, int width,
+                           const int32_t *slot, const float *weights, void *dy, float *dweights, void *workspace,
+                           size_t ws_bytes, void *stream);
 
 #ifdef __cplusplus
 }

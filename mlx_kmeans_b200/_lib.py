@@ -91,6 +91,8 @@ SIGNATURES = {
                                     _vp]),
     "kmc_combine": (_int, [_vp, _int, _i64, _int, _int, _vp, _vp, _vp, _vp]),
     "kmc_combine_grad": (_int, [_vp, _vp, _int, _i64, _int, _int, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "kmc_combine_bytes": (_sz, [_i64, _int]),
+    "kmc_combine_grad_slots": (_int, [_vp, _vp, _int, _i64, _int, _int, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
 }
 
 _lib = None

@@ -1089,13 +1089,9 @@ int kmc_combine(const void* y, int dtype, int64_t rows, int choices, int width, 
     return KMC_OK;
 }
 
-int kmc_combine_grad(const void* dout, const void* y, int dtype, int64_t rows, int choices, int width,
-                     const int32_t* slot, const float* weights, const int32_t* taken, void* dy, float* dweights,
-                     void* stream) {
-    if (int s = check_combine("kmc_combine_grad", dtype, rows, choices, width)) return s;
-    if (rows > 0 && (!dout || !slot || !taken || !dy || (dweights && !y)))
-        return fail(KMC_ERR_INVALID, "kmc_combine_grad: null pointer");
-    if (rows == 0) return KMC_OK;
+static int run_combine_grad(const char* who, const void* dout, const void* y, int dtype, int64_t rows, int choices, int width,
+                            const int32_t* slot, const float* weights, const int32_t* taken, int32_t* pair_of, void* dy,
+                            float* dweights, void* stream) {
     CombineCall c = {};
     c.y = y;
     c.slot = slot;
@@ -1106,11 +1102,42 @@ int kmc_combine_grad(const void* dout, const void* y, int dtype, int64_t rows, i
     c.dtype = dtype;
     c.dout = dout;
     c.taken = taken;
+    c.pair_of = pair_of;
     c.dy = dy;
     c.dweights = dweights;
     cudaError_t e = launch_combine(c, static_cast<cudaStream_t>(stream));
-    if (e != cudaSuccess) return cuda_fail(e, "kmc_combine_grad");
+    if (e != cudaSuccess) return cuda_fail(e, who);
     return KMC_OK;
+}
+
+int kmc_combine_grad(const void* dout, const void* y, int dtype, int64_t rows, int choices, int width,
+                     const int32_t* slot, const float* weights, const int32_t* taken, void* dy, float* dweights,
+                     void* stream) {
+    if (int s = check_combine("kmc_combine_grad", dtype, rows, choices, width)) return s;
+    if (rows > 0 && (!dout || !slot || !taken || !dy || (dweights && !y)))
+        return fail(KMC_ERR_INVALID, "kmc_combine_grad: null pointer");
+    if (rows == 0) return KMC_OK;
+    return run_combine_grad("kmc_combine_grad", dout, y, dtype, rows, choices, width, slot, weights, taken, nullptr, dy,
+                            dweights, stream);
+}
+
+size_t kmc_combine_bytes(int64_t rows, int choices) {
+    return rows > 0 && choices > 0 && rows <= INT32_MAX / choices ? (size_t)rows * choices * sizeof(int32_t) : 0;
+}
+
+int kmc_combine_grad_slots(const void* dout, const void* y, int dtype, int64_t rows, int choices, int width,
+                           const int32_t* slot, const float* weights, void* dy, float* dweights, void* workspace,
+                           size_t ws_bytes, void* stream) {
+    if (int s = check_combine("kmc_combine_grad_slots", dtype, rows, choices, width)) return s;
+    if (rows > 0 && (!dout || !slot || !dy || (dweights && !y)))
+        return fail(KMC_ERR_INVALID, "kmc_combine_grad_slots: null pointer");
+    if (rows == 0) return KMC_OK;
+    const size_t need = kmc_combine_bytes(rows, choices);
+    if (!workspace || ws_bytes < need)
+        return fail(KMC_ERR_INVALID, "kmc_combine_grad_slots: workspace of %zu bytes, need %zu",
+                    workspace ? ws_bytes : (size_t)0, need);
+    return run_combine_grad("kmc_combine_grad_slots", dout, y, dtype, rows, choices, width, slot, weights, nullptr,
+                            static_cast<int32_t*>(workspace), dy, dweights, stream);
 }
 
 }  // extern "C"

@@ -209,6 +209,8 @@ struct Groups {
 
 // ---------------------------------------------------------------- combination
 
+Tensor workspace(size_t need, const Tensor& like) { return need ? empty({(int64_t)need}, at::kByte, like) : Tensor(); }
+
 Tensor combine_of(const Tensor& y, int type, const Groups& g, const Tensor& weights) {
     Tensor out = empty({g.T, y.size(1)}, y.scalar_type(), y);
     check(kmc_combine(data(y), type, g.T, as_int(g.k, "choices"), as_int(y.size(1), "width"), ptr<int32_t>(g.slot),
@@ -251,10 +253,13 @@ std::tuple<Tensor, Maybe> combine_grad(const Tensor& dout0, const Tensor& y0, co
     Tensor dy = empty(y.sizes(), y.scalar_type(), y);
     Maybe dw;
     if (weights0) dw = empty(weights.sizes(), at::kFloat, y);
-    check(kmc_combine_grad(data(dout), data(y), type, g.T, as_int(g.k, "choices"), as_int(y.size(1), "width"),
-                           ptr<int32_t>(slot), weights0 ? ptr<float>(weights) : nullptr, g.off() + g.E, data(dy),
-                           dw ? ptr<float>(*dw) : nullptr, stream(y)),
-          "kmc_combine_grad");
+    const int k = as_int(g.k, "choices");
+    const size_t need = kmc_combine_bytes(g.T, k);
+    const Tensor ws = workspace(need, y);
+    check(kmc_combine_grad_slots(data(dout), data(y), type, g.T, k, as_int(y.size(1), "width"), ptr<int32_t>(slot),
+                                 weights0 ? ptr<float>(weights) : nullptr, data(dy), dw ? ptr<float>(*dw) : nullptr,
+                                 need ? data(ws) : nullptr, need, stream(y)),
+          "kmc_combine_grad_slots");
     return {dy, dw};
 }
 
@@ -277,8 +282,6 @@ void check_dy(const Tensor& dy, int64_t n, at::ScalarType type, const Groups& g,
     beside(dy, "dy", like);
     if (dy.size(0) != g.P || dy.size(1) != n) refuse("dy is ", shape(dy), ", the products ", g.P, " x ", n);
 }
-
-Tensor workspace(size_t need, const Tensor& like) { return need ? empty({(int64_t)need}, at::kByte, like) : Tensor(); }
 
 Tensor expert_matmul(const Tensor& x0, const Tensor& w0, const Tensor& offsets, const Tensor& rows, const Tensor& slot,
                      bool gather) {

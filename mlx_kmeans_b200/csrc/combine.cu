@@ -1,7 +1,9 @@
 // combine.cu -- joining the experts' answers (kmc_combine) and its gradient (kmc_combine_grad).
 //
 //   out_t = sum_j w_tj y_slot(t,j)          dy_slot(t,j) = w_tj dout_t          dw_tj = <dout_t, y_slot(t,j)>
-// w = 1 without weights; a pair with slot -1 adds nothing (dw 0), and a row of dy that no pair has is 0.  Sums run in
+// w = 1 without weights; a pair with slot -1 adds nothing (dw 0), and a row of dy that no pair has is 0.  Which rows those
+// are is found from the slots, in a launch before (a caller may drop pairs of a plan by their slots), or from the plan's
+// offsets where the caller says that none was dropped.  Sums run in
 // float32 in the order j = 0 .. k - 1 (out) or in a fixed tree over the row (dw), and are rounded once when stored; y may
 // be float32 where out is 16-bit (a row's gradients by position, from expert_tc.cu).
 //
@@ -24,7 +26,8 @@ constexpr int kCombineThreads = 256;
 struct CombineArgs {
     const int32_t* slot;
     const float* weights;
-    const int32_t* taken;                 // device: positions that a pair has (offsets[E])
+    const int32_t* taken;                 // device: positions that a pair has (offsets[E]), or nullptr: see pair_of
+    int32_t* pair_of;                     // a pair per position, any value where there is none
     int64_t tokens, pairs;
     int choices, width;                   // width: features
 };
@@ -56,6 +59,22 @@ __global__ void __launch_bounds__(kCombineThreads) k_combine(const T* __restrict
     *reinterpret_cast<Pack<O, V>*>(out + t * a.width + f) = r;
 }
 
+// The pair of each position that has one; the others keep what they held, which has_pair sees through, so nothing is
+// cleared first.
+__global__ void __launch_bounds__(kCombineThreads) k_pair_of(CombineArgs a) {
+    pdl_wait();
+    const int64_t p = (int64_t)blockIdx.x * kCombineThreads + threadIdx.x;
+    if (p >= a.pairs) return;
+    const int64_t s = __ldg(a.slot + p);
+    if (s >= 0 && s < a.pairs) a.pair_of[s] = (int32_t)p;
+}
+// Whether some pair points at position p
+__device__ __forceinline__ bool has_pair(const CombineArgs& a, int64_t p) {
+    if (a.taken) return p < __ldg(a.taken);
+    const int64_t q = __ldcg(a.pair_of + p);
+    return q >= 0 && q < a.pairs && __ldg(a.slot + q) == p;
+}
+
 template <typename T, int V>
 __global__ void __launch_bounds__(kCombineThreads)
     k_combine_grad(const T* __restrict__ dout, const T* __restrict__ y, CombineArgs a, T* __restrict__ dy,
@@ -65,7 +84,7 @@ __global__ void __launch_bounds__(kCombineThreads)
     const int64_t p = (int64_t)blockIdx.x * (kCombineThreads / 32) + (threadIdx.x >> 5);
     if (p >= a.pairs) return;
     const int64_t s = __ldg(a.slot + p);
-    if (p >= __ldg(a.taken)) {            // position p has no pair: its row of dy is 0
+    if (!has_pair(a, p)) {                // its row of dy is 0
         for (int f = lane * V; f < a.width; f += 32 * V) {
             Pack<T, V> z;
 #pragma unroll
@@ -105,6 +124,7 @@ cudaError_t run_combine(const CombineCall& c, cudaStream_t st) {
     a.slot = c.slot;
     a.weights = c.weights;
     a.taken = c.taken;
+    a.pair_of = c.pair_of;
     a.tokens = c.tokens;
     a.pairs = c.tokens * c.choices;
     a.choices = c.choices;
@@ -115,6 +135,10 @@ cudaError_t run_combine(const CombineCall& c, cudaStream_t st) {
                           static_cast<const T*>(c.y), a, static_cast<O*>(c.out));
     }
     if constexpr (std::is_same<T, O>::value) {
+        if (!a.taken) {
+            const int64_t blocks = (a.pairs + kCombineThreads - 1) / kCombineThreads;
+            if (cudaError_t e = launch_pdl(k_pair_of, dim3((unsigned)blocks), dim3(kCombineThreads), 0, st, a)) return e;
+        }
         const int64_t blocks = (a.pairs + kCombineThreads / 32 - 1) / (kCombineThreads / 32);
         return launch_pdl(k_combine_grad<T, V>, dim3((unsigned)blocks), dim3(kCombineThreads), 0, st,
                           static_cast<const T*>(c.dout), static_cast<const T*>(c.y), a, static_cast<T*>(c.dy),

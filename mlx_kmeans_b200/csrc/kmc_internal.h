@@ -267,7 +267,8 @@ struct CombineCall {
     int sum_f32;              // forward, dtype 16-bit: y is float32 and rounded in out for the first time
     void* out;                // forward: tokens x width
     const void* dout;         // gradient (nullptr: forward)
-    const int32_t* taken;     // device: positions with a pair
+    const int32_t* taken;     // device: positions with a pair, all below it; or nullptr: found from the slots, in pair_of
+    int32_t* pair_of;         // tokens x choices, uninitialised
     void* dy;
     float* dweights;          // or nullptr
 };

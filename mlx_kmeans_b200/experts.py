@@ -42,7 +42,8 @@ class RowGroups(NamedTuple):
 
     offsets (n_experts + 1): expert e has the positions offsets[e] .. offsets[e + 1] - 1.
     rows (pairs): the row each position reads, -1 past offsets[-1].
-    slot (rows, choices) or (rows,): the position of each pair, -1 for a pair that was left out.
+    slot (rows, choices) or (rows,): the position of each pair, -1 for a pair that was left out.  A caller may set
+    further ones to -1 (experts over their capacity): combine_rows and the gradients then leave those pairs out.
     """
     offsets: torch.Tensor
     rows: torch.Tensor

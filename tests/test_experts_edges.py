@@ -21,3 +21,19 @@ def test_dx_rows_arguments():
     assert L.kmc_expert_dx_rows_bytes(P, P, 4, 1, 4, 8, 16) == 256                  # 16-bit: nothing is summed
     assert L.kmc_expert_dx_rows_bytes(P, P, 4, 2, 4, 8, 15) == 512 + 4 * 8 * 16 * 2  # and W's rows padded
     assert call(rows=0, dy=None, slot=None, dx=None, ws=None, nb=0) == _l.KMC_OK
+
+
+def test_combine_grad_slots_arguments():
+    _l, L = lib()
+    bad, no = _l.KMC_ERR_INVALID, _l.KMC_ERR_UNSUPPORTED
+
+    def call(dout=P, y=P, dtype=0, rows=4, choices=2, width=8, slot=P, dy=P, dw=P, ws=P, nb=32):
+        return L.kmc_combine_grad_slots(dout, y, dtype, rows, choices, width, slot, None, dy, dw, ws, nb, None)
+
+    assert call(dtype=3) == bad and call(rows=-1) == bad and call(choices=0) == bad and call(width=0) == bad
+    assert call(rows=2 ** 31, choices=1) == no and call(width=(1 << 20) + 1) == no
+    for missing in ("dout", "y", "slot", "dy"):
+        assert call(**{missing: None}) == bad and b"null" in L.kmc_last_error()
+    assert L.kmc_combine_bytes(4, 2) == 32 and L.kmc_combine_bytes(0, 2) == 0 and L.kmc_combine_bytes(2 ** 31, 1) == 0
+    assert call(nb=31) == bad and b"workspace" in L.kmc_last_error() and call(ws=None) == bad
+    assert call(rows=0, dout=None, y=None, slot=None, dy=None, ws=None, nb=0) == _l.KMC_OK

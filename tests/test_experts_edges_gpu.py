@@ -146,3 +146,48 @@ def test_dx_of_labels_and_of_single_choices():
         _, (rx, xm), _ = ref_matmul(x, w, groups, True, dy)
         near(dx, by_row(groups, rx), by_row(groups, xm), 40)
         assert int(dx[lab.reshape(-1).cuda() < 0].abs().max()) == 0
+
+
+# ---------------------------------------------------------------- pairs dropped after the grouping
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("weighted", [True, False])
+@pytest.mark.parametrize("T,k,H", [(1, 1, 1), (1, 8, 64), (3, 2, 33), (130, 8, 515), (40, 3, 2048), (2500, 4, 24)])
+def test_combine_grad_of_positions_without_a_pair(T, k, H, weighted, dt):
+    """Slots set to -1 after the grouping (experts over their capacity): their positions' rows of dy are zeros, and
+    dW, which sums positions by the offsets, gets nothing from them."""
+    from mlx_kmeans_b200 import combine_rows_grad, expert_matmul_grad
+    E = max(4, k)
+    groups = plan(T, k, E, T + H, drop=0.1)
+    g = rng(H)
+    groups.slot[(torch.rand(T, k, generator=g) < 0.3).cuda()] = -1
+    if T > 2:
+        groups.slot[1] = -1
+    y, dout = torch.randn(T * k, H, generator=g).to(dt).cuda(), torch.randn(T, H, generator=g).to(dt).cuda()
+    w = torch.rand(T, k, generator=g).cuda() if weighted else None
+    stale = torch.full_like(y, float("nan"))
+    del stale                                                 # the allocator's next block of this size
+    dy, dw = combine_rows_grad(dout, y, groups, w)
+    slot = groups.slot.cpu().long()
+    wv = (w.double().cpu() if weighted else torch.ones(T, k, dtype=torch.float64))[:, :, None]
+    ref = torch.zeros(T * k, H, dtype=torch.float64)
+    ref[slot[slot >= 0]] = (wv * dout.double().cpu()[:, None, :]).expand(T, k, H)[slot >= 0]
+    near(dy, ref, ref.abs(), 1)
+    assert torch.all(dy.cpu()[ref.abs().sum(1) == 0] == 0)
+    if weighted:
+        assert torch.all(dw[groups.slot < 0] == 0)
+    if dt in HALF and H > 1:
+        x, m = torch.randn(T, 16, generator=g).to(dt).cuda(), torch.zeros(E, H, 16, dtype=dt, device="cuda")
+        _, _, (rw, wm) = ref_matmul(x, m, groups, True, dy)
+        near(expert_matmul_grad(dy, x, m, groups)[1], rw, wm, T * k)
+
+
+def test_combine_grad_where_rows_and_slots_disagree():
+    """dy follows the slots alone: a position whose row entry was changed keeps its gradient."""
+    from mlx_kmeans_b200 import RowGroups, combine_rows_grad, group_rows
+    ids = torch.tensor([[0, 1], [1, 2], [0, 2]], dtype=torch.int32).cuda()
+    groups = group_rows(ids, 3)
+    y, dout = torch.ones(6, 8).cuda(), torch.arange(1.0, 4.0)[:, None].expand(3, 8).contiguous().cuda()
+    want, _ = combine_rows_grad(dout, y, groups)
+    odd = RowGroups(groups.offsets, torch.full_like(groups.rows, 99), groups.slot)
+    assert torch.equal(combine_rows_grad(dout, y, odd)[0], want) and bool((want != 0).all())
