@@ -9,7 +9,8 @@ centers (or any gate's scores) on to a mixture of experts:
     out = combine_rows(y, groups, weights)         # a row's results summed with its weights
 
 All arguments are CUDA tensors; work is enqueued on the current stream and nothing synchronises.  route,
-expert_matmul and combine_rows are differentiable through torch.autograd; route_grad, expert_matmul_grad and
+expert_matmul and combine_rows are differentiable through torch.autograd, once: their gradients have no derivative of
+their own, and asking for one (create_graph) is a RuntimeError.  route_grad, expert_matmul_grad and
 combine_rows_grad are the same gradients as plain calls.  group_rows takes labels too (KMeans.labels_ on the device),
 to run one product per cluster.  Errors: ValueError for bad arguments, RuntimeError for a device failure.
 Calls can be captured in a CUDA graph, except a device's first expert_matmul (it allocates the word expert_status reads).
@@ -65,6 +66,27 @@ def expert_status(device=None):
         raise RuntimeError("expert_matmul: a kernel gave up waiting on a barrier; its result is incomplete")
 
 
+class _Last(torch.autograd.Function):
+    """Gradients tied to everything they depend on, so that a derivative taken through them is refused, whichever of
+    those it is asked for."""
+    @staticmethod
+    def forward(ctx, n, *tensors):
+        return tuple(t.view_as(t) for t in tensors[:n])
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("route, expert_matmul and combine_rows have no second derivative")
+
+
+def _last(grads, *sources):
+    """The gradients of a backward pass (None where there is none), made from `sources`."""
+    if not torch.is_grad_enabled():                            # create_graph is not set
+        return grads
+    some = [g for g in grads if g is not None]
+    done = iter(_Last.apply(len(some), *some, *sources)) if some else iter(())
+    return tuple(None if g is None else next(done) for g in grads)
+
+
 # ---------------------------------------------------------------- routing
 
 def _route_flags(score, renormalize):
@@ -86,7 +108,7 @@ class _Route(torch.autograd.Function):
     def backward(ctx, _dids, dweights):
         logits, ids = ctx.saved_tensors
         dl = _ext().route_grad(dweights.float(), logits, ids, ctx.flags, ctx.scale)
-        return dl, None, None, None, None, None, None, None
+        return (*_last((dl,), dweights, logits), None, None, None, None, None, None, None)
 
 
 def route(logits, top_k, *, score="softmax", bias=None, groups=1, top_groups=1, renormalize=True, scale=1.0, mask=None):
@@ -144,7 +166,7 @@ class _ExpertMatmul(torch.autograd.Function):
         x, w, offsets, rows, slot = ctx.saved_tensors
         dx = _ext().expert_dx(dy, w, offsets, rows, slot, ctx.gather) if ctx.needs_input_grad[0] else None
         dw = _ext().expert_dw(dy, x, offsets, rows, slot, ctx.gather) if ctx.needs_input_grad[1] else None
-        return dx, dw, None, None, None, None
+        return (*_last((dx, dw), dy, x, w), None, None, None, None)
 
 
 def expert_matmul(x, w, groups, *, gather=True):
@@ -180,7 +202,7 @@ class _Combine(torch.autograd.Function):
     def backward(ctx, dout):
         y, weights, offsets, rows, slot = ctx.saved_tensors
         dy, dw = _ext().combine_grad(dout, y, offsets, rows, slot, weights)
-        return dy, dw, None, None, None
+        return (*_last((dy, dw), dout, y, *(() if weights is None else (weights,))), None, None, None)
 
 
 def combine_rows(y, groups, weights: Optional[torch.Tensor] = None):

@@ -191,3 +191,49 @@ def test_combine_grad_where_rows_and_slots_disagree():
     want, _ = combine_rows_grad(dout, y, groups)
     odd = RowGroups(groups.offsets, torch.full_like(groups.rows, 99), groups.slot)
     assert torch.equal(combine_rows_grad(dout, y, odd)[0], want) and bool((want != 0).all())
+
+
+# ---------------------------------------------------------------- derivatives of the derivatives
+
+def _differentiable_calls():
+    """name -> (function of its float inputs, those inputs)."""
+    from mlx_kmeans_b200 import combine_rows, expert_matmul, group_rows, route
+    g = rng(12)
+    ids = torch.stack([torch.randperm(4, generator=g)[:2] for _ in range(6)]).to(torch.int32).cuda()
+    groups = group_rows(ids, 4)
+    l, y, c = torch.randn(6, 4, generator=g).cuda(), torch.randn(12, 8, generator=g).cuda(), torch.rand(6, 2, generator=g).cuda()
+    x, w = torch.randn(6, 16, generator=g).half().cuda(), torch.randn(4, 8, 16, generator=g).half().cuda()
+    return {"route": (lambda l: route(l, 2, renormalize=False)[1], [l]),
+            "expert_matmul": (lambda x, w: expert_matmul(x, w, groups), [x, w]),
+            "combine_rows": (lambda y, c: combine_rows(y, groups, c), [y, c])}
+
+
+@pytest.mark.parametrize("name", ["route", "expert_matmul", "combine_rows"])
+def test_second_derivatives_are_refused(name):
+    """The gradients have no derivative of their own: a loss made from them raises, beside other terms too, whether or
+    not the gradient that came in had one, and whichever input's derivative is asked for."""
+    f, args = _differentiable_calls()[name]
+    for loss in (lambda v: v.float().sum(), lambda v: v.float().square().sum()):
+        for i in range(len(args)):
+            ins = [a.clone().requires_grad_(True) for a in args]
+            grads = torch.autograd.grad(loss(f(*ins)), ins, create_graph=True)
+            penalty = grads[i].float().square().sum() + sum(a.float().square().sum() for a in ins)
+            with pytest.raises(RuntimeError, match="second derivative"):
+                torch.autograd.grad(penalty, ins)
+            ins = [a.clone().requires_grad_(True) for a in args]
+            grads = torch.autograd.grad(loss(f(*ins)), ins, create_graph=True)
+            with pytest.raises(RuntimeError, match="second derivative"):
+                (grads[i].float().square().sum() + sum(a.float().square().sum() for a in ins)).backward()
+
+
+@pytest.mark.parametrize("name", ["route", "expert_matmul", "combine_rows"])
+def test_first_derivatives_with_a_graph_kept(name):
+    """create_graph alone changes no gradient, and one that is not differentiated again raises nothing."""
+    f, args = _differentiable_calls()[name]
+    ins = [a.clone().requires_grad_(True) for a in args]
+    plain = torch.autograd.grad(f(*ins).float().square().sum(), ins)
+    kept = torch.autograd.grad(f(*ins).float().square().sum(), ins, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, kept))
+    only = args[0].clone().requires_grad_(True)               # one input alone
+    kept, = torch.autograd.grad(f(only, *args[1:]).float().square().sum(), [only], create_graph=True)
+    assert torch.equal(kept, plain[0])
