@@ -47,6 +47,11 @@ void on_gpu(const Tensor& t, const char* name, int64_t ndim = -1) {
 void beside(const Tensor& t, const char* name, const Tensor& other) {
     if (t.device() != other.device()) refuse(name, " is on ", t.device(), ", not on ", other.device());
 }
+// An input whose derivative counts carries no tangent of forward-mode differentiation, which would be lost here.
+void no_tangent(const Tensor& t, const char* name) {
+    if (t._fw_grad(0).defined())
+        throw std::runtime_error(std::string("route, expert_matmul and combine_rows have no forward-mode derivative (") + name + " has a tangent)");
+}
 void of_type(const Tensor& t, const char* name, at::ScalarType type) {
     if (t.scalar_type() != type) refuse(name, " must be ", type, ", got ", t.scalar_type());
 }
@@ -113,6 +118,7 @@ bool status(int64_t device) {
 std::tuple<Tensor, Tensor> route(const Tensor& logits0, int64_t top_k, int64_t flags, const Maybe& bias0, int64_t groups,
                                  int64_t top_groups, double scale, const Maybe& mask0) {
     on_gpu(logits0, "logits", 2);
+    no_tangent(logits0, "logits");
     const int type = dtype_of(logits0, "logits", true);
     const Tensor logits = rows_of(logits0);
     const int64_t T = logits.size(0), E = logits.size(1);
@@ -144,11 +150,13 @@ std::tuple<Tensor, Tensor> route(const Tensor& logits0, int64_t top_k, int64_t f
 
 Tensor route_grad(const Tensor& dweights, const Tensor& logits0, const Tensor& ids, int64_t flags, double scale) {
     on_gpu(logits0, "logits", 2);
+    no_tangent(logits0, "logits");
     const int type = dtype_of(logits0, "logits", true);
     on_gpu(ids, "ids", 2);
     of_type(ids, "ids", at::kInt);
     beside(ids, "ids", logits0);
     on_gpu(dweights, "dweights", 2);
+    no_tangent(dweights, "dweights");
     of_type(dweights, "dweights", at::kFloat);
     beside(dweights, "dweights", logits0);
     if (ids.sizes() != dweights.sizes() || ids.size(0) != logits0.size(0))
@@ -222,6 +230,7 @@ Tensor combine_of(const Tensor& y, int type, const Groups& g, const Tensor& weig
 Tensor weights_of(const Maybe& weights, const Groups& g, const Tensor& y) {
     if (!weights) return {};
     on_gpu(*weights, "weights");
+    no_tangent(*weights, "weights");
     of_type(*weights, "weights", at::kFloat);
     beside(*weights, "weights", y);
     if (weights->sizes() != g.slot.sizes()) refuse("weights are ", shape(*weights), ", the groups' pairs ", shape(g.slot));
@@ -230,6 +239,7 @@ Tensor weights_of(const Maybe& weights, const Groups& g, const Tensor& y) {
 
 Tensor combine(const Tensor& y0, const Tensor& offsets, const Tensor& rows, const Tensor& slot, const Maybe& weights) {
     on_gpu(y0, "y", 2);
+    no_tangent(y0, "y");
     const int type = dtype_of(y0, "y", true);
     const Groups g(offsets, rows, slot, y0);
     if (y0.size(0) != g.P) refuse("y has ", y0.size(0), " rows for ", g.P, " positions");
@@ -240,10 +250,12 @@ Tensor combine(const Tensor& y0, const Tensor& offsets, const Tensor& rows, cons
 std::tuple<Tensor, Maybe> combine_grad(const Tensor& dout0, const Tensor& y0, const Tensor& offsets, const Tensor& rows,
                                        const Tensor& slot, const Maybe& weights0) {
     on_gpu(y0, "y", 2);
+    no_tangent(y0, "y");
     const int type = dtype_of(y0, "y", true);
     const Groups g(offsets, rows, slot, y0);
     if (y0.size(0) != g.P) refuse("y has ", y0.size(0), " rows for ", g.P, " positions");
     on_gpu(dout0, "dout", 2);
+    no_tangent(dout0, "dout");
     of_type(dout0, "dout", y0.scalar_type());
     beside(dout0, "dout", y0);
     if (dout0.size(0) != g.T || dout0.size(1) != y0.size(1))
@@ -267,6 +279,7 @@ std::tuple<Tensor, Maybe> combine_grad(const Tensor& dout0, const Tensor& y0, co
 
 void check_x(const Tensor& x, int64_t d, at::ScalarType type, const Groups& g, bool gather) {
     on_gpu(x, "x", 2);
+    no_tangent(x, "x");
     of_type(x, "x", type);
     if (x.size(1) != d) refuse("x has ", x.size(1), " columns, the matrices ", d);
     const int64_t want = gather ? g.T : g.P;
@@ -278,6 +291,7 @@ int check_w(const Tensor& w, const Groups& g) {
 }
 void check_dy(const Tensor& dy, int64_t n, at::ScalarType type, const Groups& g, const Tensor& like) {
     on_gpu(dy, "dy", 2);
+    no_tangent(dy, "dy");
     of_type(dy, "dy", type);
     beside(dy, "dy", like);
     if (dy.size(0) != g.P || dy.size(1) != n) refuse("dy is ", shape(dy), ", the products ", g.P, " x ", n);
@@ -286,6 +300,7 @@ void check_dy(const Tensor& dy, int64_t n, at::ScalarType type, const Groups& g,
 Tensor expert_matmul(const Tensor& x0, const Tensor& w0, const Tensor& offsets, const Tensor& rows, const Tensor& slot,
                      bool gather) {
     on_gpu(w0, "w", 3);
+    no_tangent(w0, "w");
     const Groups g(offsets, rows, slot, w0);
     const int type = check_w(w0, g);
     check_x(x0, w0.size(2), w0.scalar_type(), g, gather);
@@ -306,6 +321,7 @@ Tensor expert_matmul(const Tensor& x0, const Tensor& w0, const Tensor& offsets, 
 Tensor expert_dx(const Tensor& dy0, const Tensor& w0, const Tensor& offsets, const Tensor& rows, const Tensor& slot,
                  bool gather) {
     on_gpu(w0, "w", 3);
+    no_tangent(w0, "w");
     const Groups g(offsets, rows, slot, w0);
     const int type = check_w(w0, g);
     check_dy(dy0, w0.size(1), w0.scalar_type(), g, w0);

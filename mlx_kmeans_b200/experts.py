@@ -10,8 +10,8 @@ centers (or any gate's scores) on to a mixture of experts:
 
 All arguments are CUDA tensors; work is enqueued on the current stream and nothing synchronises.  route,
 expert_matmul and combine_rows are differentiable through torch.autograd, once: their gradients have no derivative of
-their own, and asking for one (create_graph) is a RuntimeError.  route_grad, expert_matmul_grad and
-combine_rows_grad are the same gradients as plain calls.  group_rows takes labels too (KMeans.labels_ on the device),
+their own, and asking for one (create_graph) is a RuntimeError, as is forward-mode differentiation.  route_grad,
+expert_matmul_grad and combine_rows_grad are the same gradients as plain calls.  group_rows takes labels too (KMeans.labels_ on the device),
 to run one product per cluster.  Errors: ValueError for bad arguments, RuntimeError for a device failure.
 Calls can be captured in a CUDA graph, except a device's first expert_matmul (it allocates the word expert_status reads).
 """
@@ -66,6 +66,13 @@ def expert_status(device=None):
         raise RuntimeError("expert_matmul: a kernel gave up waiting on a barrier; its result is incomplete")
 
 
+class _Once(torch.autograd.Function):
+    """A function with a backward pass alone."""
+    @staticmethod
+    def jvp(ctx, *_):
+        raise RuntimeError("route, expert_matmul and combine_rows have no forward-mode derivative")
+
+
 class _Last(torch.autograd.Function):
     """Gradients tied to everything they depend on, so that a derivative taken through them is refused, whichever of
     those it is asked for."""
@@ -95,7 +102,7 @@ def _route_flags(score, renormalize):
     return _SCORES[score] | (_lib.KMC_ROUTE_RENORM if renormalize else 0)
 
 
-class _Route(torch.autograd.Function):
+class _Route(_Once):
     @staticmethod
     def forward(ctx, logits, top_k, flags, bias, groups, top_groups, scale, mask):
         ids, weights = _ext().route(logits, top_k, flags, bias, groups, top_groups, scale, mask)
@@ -154,7 +161,7 @@ def group_rows(ids, n_experts):
 
 # ---------------------------------------------------------------- products per expert
 
-class _ExpertMatmul(torch.autograd.Function):
+class _ExpertMatmul(_Once):
     @staticmethod
     def forward(ctx, x, w, offsets, rows, slot, gather):
         ctx.save_for_backward(x, w, offsets, rows, slot)
@@ -192,7 +199,7 @@ def expert_matmul_grad(dy, x, w, groups, *, gather=True):
 
 # ---------------------------------------------------------------- combination
 
-class _Combine(torch.autograd.Function):
+class _Combine(_Once):
     @staticmethod
     def forward(ctx, y, weights, offsets, rows, slot):
         ctx.save_for_backward(y, weights, offsets, rows, slot)

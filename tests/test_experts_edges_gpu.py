@@ -237,3 +237,37 @@ def test_first_derivatives_with_a_graph_kept(name):
     only = args[0].clone().requires_grad_(True)               # one input alone
     kept, = torch.autograd.grad(f(only, *args[1:]).float().square().sum(), [only], create_graph=True)
     assert torch.equal(kept, plain[0])
+
+
+@pytest.mark.parametrize("requires", [False, True])
+@pytest.mark.parametrize("name", ["route", "expert_matmul", "combine_rows"])
+def test_forward_mode_is_refused(name, requires):
+    """A tangent is not dropped: the functions have no forward-mode derivative and say so."""
+    import torch.autograd.forward_ad as fw
+    f, args = _differentiable_calls()[name]
+    for i in range(len(args)):
+        with fw.dual_level():
+            ins = [a.clone().requires_grad_(requires) for a in args]
+            ins[i] = fw.make_dual(ins[i], torch.ones_like(ins[i]))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                f(*ins)
+        assert torch.isfinite(f(*args).float()).all()         # without a tangent as before
+
+
+def test_forward_mode_of_the_gradients_is_refused():
+    import torch.autograd.forward_ad as fw
+    from mlx_kmeans_b200 import combine_rows_grad, expert_matmul_grad, group_rows, route_grad
+    ids = torch.tensor([[0, 1], [1, 2]], dtype=torch.int32).cuda()
+    groups = group_rows(ids, 3)
+    half = lambda *s: torch.ones(*s, dtype=torch.float16, device="cuda")  # noqa: E731
+    full = lambda *s: torch.ones(*s, device="cuda")                      # noqa: E731
+    calls = [(lambda a, b: route_grad(a, b, ids), [full(2, 2), full(2, 3)]),
+             (lambda a, b, c: expert_matmul_grad(a, b, c, groups), [half(4, 8), half(2, 16), half(3, 8, 16)]),
+             (lambda a, b, c: combine_rows_grad(a, b, groups, c), [full(2, 8), full(4, 8), full(2, 2)])]
+    for f, args in calls:
+        for i in range(len(args)):
+            with fw.dual_level():
+                ins = list(args)
+                ins[i] = fw.make_dual(ins[i], torch.ones_like(ins[i]))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    f(*ins)
