@@ -378,8 +378,9 @@ int kmc_group_rows(const int32_t *ids, int64_t rows, int choices, int experts, i
  * kmc_expert_matmul_dw: dW (experts x n x d) = sum over an expert's positions of dy x^T; 0 for an expert with none.
  * workspace: kmc_expert_bytes bytes for the call's operands (NULL for one it does not take), 256-byte aligned: room for
  * x in grouped order where that is read faster, and for padded copies of operands that do not start on 16 bytes or have
- * rows that are not a multiple of 8 elements apart; may be 0.  error (device int32, set to 0 once by the
- * caller): 1 once a kernel gave up waiting on a barrier, its output then incomplete. */
+ * rows that are not a multiple of 8 elements apart; may be 0.  error (an int32 that the device can
+ * write, in its memory or the host's, set to 0 once by the caller): 1 once a kernel gave up waiting on a barrier, its
+ * output then incomplete. */
 size_t kmc_expert_bytes(const void *x, int64_t x_rows, int64_t ldx, const int32_t *group_row, const void *w,
                         const void *dy, int64_t pairs, int experts, int n, int d);
 int kmc_expert_matmul(const void *x, int64_t x_rows, int64_t ldx, const int32_t *group_row, const void *w,

@@ -5,6 +5,7 @@
 // ValueError; so do statuses KMC_ERR_INVALID and KMC_ERR_UNSUPPORTED, any other status raises RuntimeError.  Work goes
 // to the current stream of the tensors' device; nothing synchronises but status().
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -87,29 +88,38 @@ int as_int(int64_t v, const char* name) {
     return (int)v;
 }
 
-// Per device: the int32 a kernel sets when it gave up on a barrier; allocated and zeroed at its first use.
+// Per device: the int32 a kernel sets when it gave up on a barrier.  It lies in pinned host memory, which the host clears
+// at its first use without a stream, so that use may be inside a graph capture (whose mode is relaxed for the
+// allocation); and it stays for the life of the process, as a graph may keep its address.
 std::mutex g_mutex;
-std::vector<Tensor> g_error(64);
+std::vector<Tensor>& error_words() {
+    static auto* words = new std::vector<Tensor>(64);
+    return *words;
+}
 
 int32_t* error_word(const Tensor& like) {
     const int i = like.device().index();
     std::lock_guard<std::mutex> lock(g_mutex);
-    if (!g_error[i].defined()) {
-        g_error[i] = at::zeros({1}, like.options().dtype(at::kInt).requires_grad(false));
-        c10::cuda::getCurrentCUDAStream(i).synchronize();      // zero before any stream's kernel can set it
+    Tensor& word = error_words().at(i);
+    if (!word.defined()) {
+        const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+        const Tensor fresh = at::empty({1}, at::TensorOptions(at::kInt).pinned_memory(true));
+        *ptr<int32_t>(fresh) = 0;
+        word = fresh;
     }
-    return ptr<int32_t>(g_error[i]);
+    return ptr<int32_t>(word);
 }
 
 bool status(int64_t device) {
-    Tensor e;
+    volatile int32_t* word;
     {
         std::lock_guard<std::mutex> lock(g_mutex);
-        if (device < 0 || device >= (int64_t)g_error.size() || !g_error[device].defined()) return false;
-        e = g_error[device];
+        if (device < 0 || device >= (int64_t)error_words().size() || !error_words()[device].defined()) return false;
+        word = ptr<int32_t>(error_words()[device]);
     }
-    const bool set = e.item<int>() != 0;
-    if (set) e.zero_();
+    c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).synchronize();
+    const bool set = *word != 0;
+    if (set) *word = 0;
     return set;
 }
 

@@ -606,7 +606,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * COLS));
         else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * COLS));
     }
-    if (threadIdx.x == 0 && *abort_flag) atomicExch(a.error, 1);
+    if (threadIdx.x == 0 && *abort_flag) *static_cast<volatile int*>(a.error) = 1;
 }
 
 // ---------------------------------------------------------------- host side

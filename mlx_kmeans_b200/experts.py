@@ -13,7 +13,7 @@ expert_matmul and combine_rows are differentiable through torch.autograd, once: 
 their own, and asking for one (create_graph) is a RuntimeError, as is forward-mode differentiation.  route_grad,
 expert_matmul_grad and combine_rows_grad are the same gradients as plain calls.  group_rows takes labels too (KMeans.labels_ on the device),
 to run one product per cluster.  Errors: ValueError for bad arguments, RuntimeError for a device failure.
-Calls can be captured in a CUDA graph, except a device's first expert_matmul (it allocates the word expert_status reads).
+Calls can be captured in a CUDA graph.
 """
 import os
 from typing import NamedTuple, Optional

@@ -271,3 +271,27 @@ def test_forward_mode_of_the_gradients_is_refused():
                 ins[i] = fw.make_dual(ins[i], torch.ones_like(ins[i]))
                 with pytest.raises(RuntimeError, match="forward-mode"):
                     f(*ins)
+
+
+# ---------------------------------------------------------------- the error word
+
+def test_first_call_of_a_process_can_be_captured():
+    """A process whose first expert_matmul is inside a graph capture: the graph replays, and no fault is reported."""
+    code = """
+        import torch
+        from mlx_kmeans_b200 import expert_matmul, expert_status, group_rows
+        torch.manual_seed(0)
+        x, w = torch.randn(40, 64, device="cuda").half(), torch.randn(4, 48, 64, device="cuda").half()
+        groups = group_rows((torch.arange(80, device="cuda").reshape(40, 2) % 4).int(), 4)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = expert_matmul(x, w, groups)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, expert_matmul(x, w, groups))
+        expert_status()
+        print("captured")
+    """
+    r = subprocess.run([sys.executable, "-c", textwrap.dedent(code)], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr
