@@ -97,8 +97,9 @@ std::vector<Tensor>& error_words() {
     return *words;
 }
 
-int32_t* error_word(const Tensor& like) {
-    const int i = like.device().index();
+const char* kGaveUp = "expert_matmul: a kernel gave up waiting on a barrier; its result is incomplete";
+
+Tensor error_tensor(int64_t i) {
     std::lock_guard<std::mutex> lock(g_mutex);
     Tensor& word = error_words().at(i);
     if (!word.defined()) {
@@ -107,20 +108,30 @@ int32_t* error_word(const Tensor& like) {
         *ptr<int32_t>(fresh) = 0;
         word = fresh;
     }
-    return ptr<int32_t>(word);
+    return word;
+}
+// The word of a call on the device of `like`; an earlier kernel's that is set raises first, and is cleared.  (The host
+// only looks at its memory: what a kernel still running has not written yet, the next call sees, or expert_status.)
+int32_t* error_word(const Tensor& like) {
+    int32_t* word = ptr<int32_t>(error_tensor(like.device().index()));
+    if (*static_cast<volatile int32_t*>(word) != 0) {
+        *word = 0;
+        throw std::runtime_error(std::string("an earlier ") + kGaveUp);
+    }
+    return word;
 }
 
-bool status(int64_t device) {
+void status(int64_t device) {
     volatile int32_t* word;
     {
         std::lock_guard<std::mutex> lock(g_mutex);
-        if (device < 0 || device >= (int64_t)error_words().size() || !error_words()[device].defined()) return false;
+        if (device < 0 || device >= (int64_t)error_words().size() || !error_words()[device].defined()) return;
         word = ptr<int32_t>(error_words()[device]);
     }
     c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).synchronize();
-    const bool set = *word != 0;
-    if (set) *word = 0;
-    return set;
+    if (*word == 0) return;
+    *word = 0;
+    throw std::runtime_error(kGaveUp);
 }
 
 // ---------------------------------------------------------------- routing
@@ -390,4 +401,5 @@ PYBIND11_MODULE(_experts, m) {
     m.def("combine", &combine);
     m.def("combine_grad", &combine_grad);
     m.def("status", &status);
+    m.def("error_word", &error_tensor);
 }

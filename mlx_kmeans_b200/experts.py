@@ -58,12 +58,12 @@ def _tensors(*named):
 
 
 def expert_status(device=None):
-    """Raise RuntimeError if an expert_matmul (or its gradient) on `device` gave up waiting on a barrier since the last
-    call, which leaves its result incomplete: a fault of the library or the device, since no wait depends on the data.
-    Waits for the device's current stream."""
+    """Raise RuntimeError if an expert_matmul (or its gradient) on `device` gave up waiting on a barrier and no call has
+    raised it yet, which leaves its result incomplete: a fault of the library or the device, since no wait depends on the
+    data.  Waits for the device's current stream.  A later expert_matmul or gradient on the device raises it too, once the
+    kernel has ended."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-    if _ext().status(device.index if device.index is not None else torch.cuda.current_device()):
-        raise RuntimeError("expert_matmul: a kernel gave up waiting on a barrier; its result is incomplete")
+    _ext().status(device.index if device.index is not None else torch.cuda.current_device())
 
 
 class _Once(torch.autograd.Function):

@@ -295,3 +295,22 @@ def test_first_call_of_a_process_can_be_captured():
     """
     r = subprocess.run([sys.executable, "-c", textwrap.dedent(code)], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "captured" in r.stdout, r.stderr
+
+
+def test_a_kernel_that_gave_up_is_raised_by_the_next_call():
+    """The word that a kernel sets when it gives up, set here from the host: forward and both gradients raise once."""
+    from mlx_kmeans_b200 import _experts, expert_matmul, expert_matmul_grad, expert_status, group_rows
+    groups = group_rows(torch.tensor([[0, 1], [1, 2]], dtype=torch.int32).cuda(), 3)
+    x, w = torch.ones(2, 16).half().cuda(), torch.ones(3, 8, 16).half().cuda()
+    dy = torch.ones(4, 8).half().cuda()
+    y = expert_matmul(x, w, groups)
+    torch.cuda.synchronize()
+    word = _experts.error_word(x.device.index)
+    assert word.dtype == torch.int32 and word.tolist() == [0]
+    for f in (lambda: expert_matmul(x, w, groups), lambda: expert_matmul_grad(dy, x, w, groups), lambda: expert_status(),
+              lambda: expert_matmul(x.clone().requires_grad_(True), w, groups)):
+        word[0] = 1
+        with pytest.raises(RuntimeError, match="gave up"):
+            f()
+        assert word.tolist() == [0]
+        assert torch.equal(expert_matmul(x, w, groups), y)
