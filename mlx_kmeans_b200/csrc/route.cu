@@ -11,7 +11,7 @@
 //            the sum over the chosen (0 when that sum is 0); times `scale`.
 // Gradient, with g = scale dL/dweights on the chosen (the choice itself, and so the bias, has none):
 //   softmax  dl_i = p_i ([i chosen] g_i - sum_j g_j p_j) over the available, RENORM: over the chosen, 0 elsewhere
-//   sigmoid  dl_i = g_i s_i (1 - s_i), RENORM: (g_i - sum_j g_j s_j / S) / S  s_i (1 - s_i), S = sum of the chosen s_j
+//   sigmoid  dl_i = g_i s_i (1 - s_i), RENORM: (g_i - sum_j g_j s_j / S) s_i (1 - s_i) / S, S = sum of the chosen s_j
 //
 // LANES lanes of a warp own a row: lane L holds the PER consecutive experts from L PER on (E up to LANES PER), read
 // with 16-byte loads where the row allows, their keys as order-preserving 32-bit integers (0: not available).
@@ -419,7 +419,8 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
     if (here && got) {
         float v;
         if (a.sigmoid) {
-            v = !a.renorm ? g * slope : total > 0.0f ? (g - dot) / total * slope : 0.0f;
+            // (slope / total is at most 1, where (g - dot) / total leaves float32's range at scores around 1e-38)
+            v = !a.renorm ? g * slope : total > 0.0f ? (g - dot) * (slope / total) : 0.0f;
         } else {
             v = p * (g - dot);
         }

@@ -314,3 +314,22 @@ def test_a_kernel_that_gave_up_is_raised_by_the_next_call():
             f()
         assert word.tolist() == [0]
         assert torch.equal(expert_matmul(x, w, groups), y)
+
+
+# ---------------------------------------------------------------- extreme scores
+
+@pytest.mark.parametrize("E", [2, 64, 200])
+def test_route_grad_of_very_small_sigmoids(E):
+    """Renormalised sigmoids around exp(-87): (g - dot) / S alone leaves float32's range, the gradient does not."""
+    from mlx_kmeans_b200 import route, route_grad
+    T = 40
+    l = torch.full((T, E), -95.0)
+    l[:, 0], l[:, 1] = -87.0 - torch.rand(T, generator=rng(1)), -86.5 - torch.rand(T, generator=rng(2))
+    g = torch.randn(T, 2, generator=rng(3)) * 10
+    ids, _ = route(l.cuda(), 2, score="sigmoid")
+    assert int(ids.max()) == 1
+    dl = route_grad(g.cuda(), l.cuda(), ids, score="sigmoid")
+    ref, mag = ref_route_grad(l, ids.cpu(), g, "sigmoid", True, 1.0)
+    # each sigmoid: 4 ulp (exponential, sum, quotient) and half a step of the subnormals, 2^-149 of at least exp(-88);
+    # it enters three times, and four products and quotients round
+    assert torch.all((dl.double().cpu() - ref).abs() <= (3 * (4 + 2) + 4) * 2.0 ** -23 * mag)
