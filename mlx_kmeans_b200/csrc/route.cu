@@ -409,9 +409,11 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
         total = row_sum<LANES>(total);
         p = got ? share(exp_below(lm - m), total) : 0.0f;
         dot = row_sum<LANES>(g * p);
-        const float c = row_ballot<LANES>(got) != 0u ? -dot / total : 0.0f;   // a row with no choice: 0, whatever its logits
+        const bool some = row_ballot<LANES>(got) != 0u;
+        const float c = -dot / total;
+        // (a row with no choice has a gradient of 0 whatever its logits, +inf and the NaN it makes among them)
 #pragma unroll
-        for (int i = 0; i < PER; i++) dl[i] = dl[i] != 0.0f ? c * dl[i] : 0.0f;
+        for (int i = 0; i < PER; i++) dl[i] = some && dl[i] != 0.0f ? c * dl[i] : 0.0f;
     }
     // the dense row first, then the chosen entries over it
     if (here) store_row<T, PER>(out, lane, a.experts, a.out_vec, dl);

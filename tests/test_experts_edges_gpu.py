@@ -333,3 +333,25 @@ def test_route_grad_of_very_small_sigmoids(E):
     # each sigmoid: 4 ulp (exponential, sum, quotient) and half a step of the subnormals, 2^-149 of at least exp(-88);
     # it enters three times, and four products and quotients round
     assert torch.all((dl.double().cpu() - ref).abs() <= (3 * (4 + 2) + 4) * 2.0 ** -23 * mag)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renorm", [False, True])
+@pytest.mark.parametrize("E", [8, 64, 200, 600])
+def test_route_grad_of_masked_rows_is_zero_whatever_they_hold(E, renorm, score, dt):
+    from mlx_kmeans_b200 import route, route_grad
+    T, k = 32, 2
+    l = torch.randn(T, E, generator=rng(E))
+    mask = torch.arange(T) % 2 == 0
+    for i, v in enumerate((INF, float("nan"), -INF, torch.finfo(dt).max)):
+        l[2 * i + 1, i] = v
+        l[2 * i + 9, :] = v
+    l, clean = l.to(dt).cuda(), torch.where(mask[:, None], l, 0.0).to(dt).cuda()
+    ids, w = route(l, k, score=score, renormalize=renorm, mask=mask.cuda())
+    g = torch.randn(T, k, generator=rng(1)).cuda()
+    dl = route_grad(g, l, ids, score=score, renormalize=renorm)
+    assert torch.all(w[~mask.cuda()] == 0) and torch.all(dl[~mask.cuda()] == 0)
+    ids2, w2 = route(clean, k, score=score, renormalize=renorm, mask=mask.cuda())
+    assert torch.equal(ids, ids2) and torch.equal(w, w2)
+    assert torch.equal(dl[mask.cuda()], route_grad(g, clean, ids2, score=score, renormalize=renorm)[mask.cuda()])
