@@ -38,11 +38,20 @@ __device__ __forceinline__ float unordered(unsigned u) {
 }
 __device__ __forceinline__ float sigmoid32(float l) { return __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-l))); }
 
-// exp of l - m <= 0 and the quotient of such by their sum (1 at least): the softmax's, by the hardware's exponential of
-// base 2.  Off by |x| 2^-23 + 2^-21 at most, relatively; below 2^-126 it is 0.  (The sigmoid, whose value decides a
-// choice bit for bit, takes expf and an IEEE division.)
-__device__ __forceinline__ float exp_below(float x) { return __expf(x); }
-__device__ __forceinline__ float share(float p, float total) { return __fdividef(p, total); }
+// exp of l - m <= 0 and the quotient of such by their sum (1 at least): the softmax's.  16-bit logits, of which each is
+// off by 2^-9 or 2^-12 of itself, take the hardware's exponential of base 2 and its quotient (off by |x| 2^-23 + 2^-21 at
+// most, relatively; below 2^-126 it is 0); float32 logits take expf and an IEEE division, and so does the sigmoid, whose
+// value decides a choice bit for bit.
+template <typename T>
+__device__ __forceinline__ float exp_below(float x) {
+    if constexpr (sizeof(T) == 2) return __expf(x);
+    return expf(x);
+}
+template <typename T>
+__device__ __forceinline__ float share(float p, float total) {
+    if constexpr (sizeof(T) == 2) return __fdividef(p, total);
+    return __fdiv_rn(p, total);
+}
 
 // Over the LANES lanes that share a row (aligned in the warp); every lane of the warp calls them.
 template <int LANES>
@@ -324,7 +333,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
         m = row_max<LANES>(m);
         total = 0.0f;
 #pragma unroll
-        for (int i = 0; i < PER; i++) total += l[i] > -INFINITY ? exp_below(l[i] - m) : 0.0f;
+        for (int i = 0; i < PER; i++) total += l[i] > -INFINITY ? exp_below<T>(l[i] - m) : 0.0f;
         total = row_sum<LANES>(total);
     }
     if constexpr (LANES == 32) {
@@ -345,9 +354,9 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
         }
     } else {
         if (a.renorm) m = row_max<LANES>(lm);
-        const float p = got ? exp_below(lm - m) : 0.0f;
+        const float p = got ? exp_below<T>(lm - m) : 0.0f;
         if (a.renorm) total = row_sum<LANES>(p);
-        w = got ? share(p, total) : 0.0f;
+        w = got ? share<T>(p, total) : 0.0f;
     }
     if (here && lane < a.choices) {
         ids[t * a.choices + lane] = mine;
@@ -386,9 +395,9 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
         }
     } else if (a.renorm) {
         m = row_max<LANES>(lm);
-        p = got ? exp_below(lm - m) : 0.0f;
+        p = got ? exp_below<T>(lm - m) : 0.0f;
         total = row_sum<LANES>(p);
-        p = got ? share(p, total) : 0.0f;
+        p = got ? share<T>(p, total) : 0.0f;
         dot = row_sum<LANES>(g * p);
     }
     float dl[PER];
@@ -403,11 +412,11 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
         total = 0.0f;
 #pragma unroll
         for (int i = 0; i < PER; i++) {
-            dl[i] = dl[i] > -INFINITY ? exp_below(dl[i] - m) : 0.0f;
+            dl[i] = dl[i] > -INFINITY ? exp_below<T>(dl[i] - m) : 0.0f;
             total += dl[i];
         }
         total = row_sum<LANES>(total);
-        p = got ? share(exp_below(lm - m), total) : 0.0f;
+        p = got ? share<T>(exp_below<T>(lm - m), total) : 0.0f;
         dot = row_sum<LANES>(g * p);
         const bool some = row_ballot<LANES>(got) != 0u;
         const float c = -dot / total;

@@ -355,3 +355,26 @@ def test_route_grad_of_masked_rows_is_zero_whatever_they_hold(E, renorm, score, 
     ids2, w2 = route(clean, k, score=score, renormalize=renorm, mask=mask.cuda())
     assert torch.equal(ids, ids2) and torch.equal(w, w2)
     assert torch.equal(dl[mask.cuda()], route_grad(g, clean, ids2, score=score, renormalize=renorm)[mask.cuda()])
+
+
+@pytest.mark.parametrize("renorm", [False, True])
+@pytest.mark.parametrize("E", [8, 33, 200])
+def test_softmax_of_float32_logits_far_apart(E, renorm):
+    """Whole-number logits down to 85 below the largest, so that l - m is exact: what is left are the exponential's own
+    2 ulp, the sum's and the quotient's rounding."""
+    from mlx_kmeans_b200 import route, route_grad
+    T, k = 500, 8
+    l = -torch.randint(1, 86, (T, E), generator=rng(E)).float()
+    l[:, 3] = 0.0
+    ids, w = route(l.cuda(), k, renormalize=renorm)
+    rid, rw = ref_route(l, k, "softmax", None, 1, 1, renorm, 1.0, None)
+    assert (ids.cpu().numpy() == rid).all()
+    # 2 ulp in the choice's exponential, 2 in the sum's terms, E additions, one quotient
+    tol = (2 + 2 + E / 2 + 1) * 2.0 ** -23
+    assert float(((w.cpu().double().numpy() - rw) / rw).__abs__().max()) <= tol
+    g = torch.zeros(T, k)
+    g[:, 0] = 1.0                                             # only the largest: the others' gradients are -p_i p_0
+    dl = route_grad(g.cuda(), l.cuda(), ids, renormalize=renorm).double().cpu()
+    ref, _ = ref_route_grad(l, ids.cpu(), g, "softmax", renorm, 1.0)
+    small = (ref != 0) & (l < 0)
+    assert float(((dl - ref) / ref)[small].abs().max()) <= 2 * tol + 2.0 ** -22
