@@ -11,8 +11,9 @@ centers (or any gate's scores) on to a mixture of experts:
 All arguments are CUDA tensors; work is enqueued on the current stream and nothing synchronises.  route,
 expert_matmul and combine_rows are differentiable through torch.autograd, once: their gradients have no derivative of
 their own, and asking for one (create_graph) is a RuntimeError, as is forward-mode differentiation.  route_grad,
-expert_matmul_grad and combine_rows_grad are the same gradients as plain calls.  group_rows takes labels too (KMeans.labels_ on the device),
-to run one product per cluster.  Errors: ValueError for bad arguments, RuntimeError for a device failure.
+expert_matmul_grad and combine_rows_grad are the same gradients as plain calls.  group_rows takes labels too, as an int32
+CUDA tensor -- KMeans.labels_ is a NumPy array on the host: torch.as_tensor(km.labels_).to("cuda", torch.int32) -- to run
+one product per cluster.  Errors: ValueError for bad arguments, RuntimeError for a device failure.
 Calls can be captured in a CUDA graph.
 """
 import os
@@ -154,6 +155,7 @@ def route_grad(dweights, logits, ids, *, score="softmax", renormalize=True, scal
 def group_rows(ids, n_experts):
     """Group (row, choice) pairs by expert: RowGroups of ids (rows, choices) or (rows,) int32, up to 4096 experts.
 
+    Labels are the (rows,) form.  Other integer types and host arrays are refused, not converted.
     Stable: an expert's pairs keep their order.  ids outside [0, n_experts) are left out (slot -1)."""
     _tensors((ids, "ids"))
     return RowGroups(*_ext().group_rows(ids, n_experts))

@@ -378,3 +378,22 @@ def test_softmax_of_float32_logits_far_apart(E, renorm):
     ref, _ = ref_route_grad(l, ids.cpu(), g, "softmax", renorm, 1.0)
     small = (ref != 0) & (l < 0)
     assert float(((dl - ref) / ref)[small].abs().max()) <= 2 * tol + 2.0 ** -22
+
+
+# ---------------------------------------------------------------- the library's own labels
+
+def test_group_rows_of_fitted_labels():
+    """KMeans.labels_ is a NumPy array on the host; as an int32 CUDA tensor it groups, and nothing else does."""
+    import numpy as np
+    from mlx_kmeans_b200 import KMeans, expert_matmul, group_rows
+    X = torch.randn(3000, 8, generator=rng(5)).numpy()
+    km = KMeans(n_clusters=6, random_state=0, n_init=1).fit(X)
+    labels = torch.as_tensor(km.labels_).to("cuda", torch.int32)
+    groups = group_rows(labels, 6)
+    for a, b in zip(groups, ref_groups(np.asarray(km.labels_), 6)):
+        assert np.array_equal(a.cpu().numpy(), b)
+    y = expert_matmul(torch.from_numpy(X).half().cuda(), torch.ones(6, 8, 8).half().cuda(), groups)
+    assert y.shape == (3000, 8)
+    for bad in (km.labels_, torch.as_tensor(km.labels_), labels.long()):
+        with pytest.raises(ValueError):
+            group_rows(bad, 6)
