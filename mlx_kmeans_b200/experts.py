@@ -58,6 +58,13 @@ def _tensors(*named):
             raise ValueError(f"{name} must be a CUDA tensor")
 
 
+def _plan(groups):
+    """offsets, rows and slot of a RowGroups (or a tuple of the three)."""
+    if not isinstance(groups, (tuple, list)) or len(groups) != 3 or not all(isinstance(t, torch.Tensor) for t in groups):
+        raise ValueError("groups must be a RowGroups (group_rows)")
+    return groups
+
+
 def expert_status(device=None):
     """Raise RuntimeError if an expert_matmul (or its gradient) on `device` gave up waiting on a barrier and no call has
     raised it yet, which leaves its result incomplete: a fault of the library or the device, since no wait depends on the
@@ -136,7 +143,10 @@ def route(logits, top_k, *, score="softmax", bias=None, groups=1, top_groups=1, 
     _tensors((logits, "logits"))
     flags = _route_flags(score, renormalize)
     if bias is not None:
+        _tensors((bias, "bias"))
         bias = bias.detach()
+    if mask is not None:
+        _tensors((mask, "mask"))
     args = (logits, top_k, flags, bias, groups, top_groups, scale, mask)
     if logits.requires_grad and torch.is_grad_enabled():
         return _Route.apply(*args)
@@ -185,8 +195,8 @@ def expert_matmul(x, w, groups, *, gather=True):
     w: (n_experts, n, d), bfloat16 or float16 as x; sums are float32.  Positions past groups.offsets[-1] are zero."""
     _tensors((x, "x"), (w, "w"))
     if (x.requires_grad or w.requires_grad) and torch.is_grad_enabled():
-        return _ExpertMatmul.apply(x, w, *groups, bool(gather))
-    return _ext().expert_matmul(x, w, *groups, gather)
+        return _ExpertMatmul.apply(x, w, *_plan(groups), bool(gather))
+    return _ext().expert_matmul(x, w, *_plan(groups), bool(gather))
 
 
 def expert_matmul_grad(dy, x, w, groups, *, gather=True):
@@ -195,7 +205,7 @@ def expert_matmul_grad(dy, x, w, groups, *, gather=True):
     _tensors((dy, "dy"), (x, "x"), (w, "w"))
     if x.ndim == 2 and w.ndim == 3 and x.shape[1] != w.shape[2]:
         raise ValueError(f"x has {x.shape[1]} columns, the matrices {w.shape[2]}")
-    ext = _ext()
+    ext, groups, gather = _ext(), _plan(groups), bool(gather)
     return ext.expert_dx(dy, w, *groups, gather), ext.expert_dw(dy, x, *groups, gather)
 
 
@@ -219,7 +229,8 @@ def combine_rows(y, groups, weights: Optional[torch.Tensor] = None):
 
     y: (positions, features), float32, bfloat16 or float16; weights float32 in the shape of the ids, or None for 1.
     The sum is float32, rounded once; a pair that was left out adds nothing."""
-    _tensors((y, "y"))
+    _tensors((y, "y"), (weights if weights is not None else y, "weights"))
+    groups = _plan(groups)
     if (y.requires_grad or (weights is not None and weights.requires_grad)) and torch.is_grad_enabled():
         return _Combine.apply(y, weights, *groups)
     return _ext().combine(y, *groups, weights)
@@ -228,5 +239,5 @@ def combine_rows(y, groups, weights: Optional[torch.Tensor] = None):
 def combine_rows_grad(dout, y, groups, weights: Optional[torch.Tensor] = None):
     """The gradients of combine_rows for dout (rows, features): dy in y's shape and type (zeros where no pair points)
     and dweights (None without weights)."""
-    _tensors((dout, "dout"), (y, "y"))
-    return _ext().combine_grad(dout, y, *groups, weights)
+    _tensors((dout, "dout"), (y, "y"), (weights if weights is not None else y, "weights"))
+    return _ext().combine_grad(dout, y, *_plan(groups), weights)

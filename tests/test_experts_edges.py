@@ -37,3 +37,24 @@ def test_combine_grad_slots_arguments():
     assert L.kmc_combine_bytes(4, 2) == 32 and L.kmc_combine_bytes(0, 2) == 0 and L.kmc_combine_bytes(2 ** 31, 1) == 0
     assert call(nb=31) == bad and b"workspace" in L.kmc_last_error() and call(ws=None) == bad
     assert call(rows=0, dout=None, y=None, slot=None, dy=None, ws=None, nb=0) == _l.KMC_OK
+
+
+def test_arguments_of_other_types():
+    """What is no tensor, and no plan, is a ValueError like any other bad argument."""
+    import pytest
+    import torch
+
+    from mlx_kmeans_b200 import RowGroups, combine_rows, combine_rows_grad, expert_matmul, expert_matmul_grad, route
+    t, w = torch.zeros(4, 8), torch.zeros(8, 4, 8)
+    ids = torch.zeros(4, 2, dtype=torch.int32)
+    g = RowGroups(torch.zeros(9, dtype=torch.int32), torch.zeros(8, dtype=torch.int32), ids)
+    plans = (None, g[:2], ids, RowGroups(None, g.rows, g.slot), "offsets")
+    calls = [lambda: route(t, 2, bias=[0.0] * 8), lambda: route(t, 2, mask=[True] * 4), lambda: route(t, 2, bias=0.0),
+             lambda: combine_rows(t, g, [1.0]), lambda: combine_rows_grad(t, t, g, 1.0)]
+    for p in plans:
+        calls += [lambda p=p: expert_matmul(t, w, p), lambda p=p: expert_matmul_grad(t, t, w, p),
+                  lambda p=p: combine_rows(t, p), lambda p=p: combine_rows_grad(t, t, p),
+                  lambda p=p: expert_matmul(t.clone().requires_grad_(True), w, p)]
+    for f in calls:
+        with pytest.raises(ValueError, match="CUDA tensor|RowGroups"):
+            f()
