@@ -397,3 +397,142 @@ def test_group_rows_of_fitted_labels():
     for bad in (km.labels_, torch.as_tensor(km.labels_), labels.long()):
         with pytest.raises(ValueError):
             group_rows(bad, 6)
+
+
+# ---------------------------------------------------------------- forms that only larger or rarer shapes take
+
+def _products(T, k, E, N, D, dt, ids=None, grads=False):
+    """expert_matmul of gathered rows (and its gradients) against float64."""
+    from mlx_kmeans_b200 import expert_matmul, expert_matmul_grad, group_rows
+    g = rng(T + N + D)
+    groups = plan(T, k, E, T) if ids is None else group_rows(ids.cuda(), E)
+    x = torch.randn(T, D, generator=g).to(dt).cuda()
+    w = (torch.randn(E, N, D, generator=g) / D ** 0.5).to(dt).cuda()
+    dy = torch.randn(T * k, N, generator=g).to(dt).cuda() if grads else None
+    (ry, ym), (rx, xm), (rw, wm) = ref_matmul(x, w, groups, True, dy)
+    near(expert_matmul(x, w, groups), ry, ym, D)
+    if grads:
+        dx, dw = expert_matmul_grad(dy, x, w, groups)
+        near(dx, by_row(groups, rx), by_row(groups, xm), N + k)
+        near(dw, rw, wm, max(1, int((groups.offsets[1:] - groups.offsets[:-1]).max())))
+    return x, w, groups
+
+
+@pytest.mark.parametrize("dt", HALF)
+@pytest.mark.parametrize("T,k,E,N,D", [(48, 4, 32, 1000, 1336), (40, 2, 8, 1000, 1336), (40, 2, 8, 1003, 1337),
+                                       (45, 2, 8, 600, 2048)])
+def test_products_that_gather_in_the_kernel(T, k, E, N, D, dt):
+    """4 to 12 rows an expert of large matrices: x's rows are read by their indices; a row outside x reads zeros."""
+    from mlx_kmeans_b200 import RowGroups, expert_matmul
+    ids = torch.stack([torch.randperm(E, generator=rng(T + t))[:k] for t in range(T)]).to(torch.int32)
+    ids[T // 2] = -1                                          # (pairs left out: the products' tiles end inside a group)
+    x, w, groups = _products(T, k, E, N, D, dt, ids)
+    y = expert_matmul(x, w, groups)
+    taken = int(groups.offsets[-1])
+    assert taken == (T - 1) * k and int(y[taken:].abs().max()) == 0
+    rows = groups.rows.clone()
+    out = torch.tensor([0, taken // 2, taken - 1])
+    rows[out.cuda()] = torch.tensor([T, -7, 2 ** 31 - 1], dtype=torch.int32).cuda()
+    y2 = expert_matmul(x, w, RowGroups(groups.offsets, rows, groups.slot))
+    keep = torch.ones(T * k, dtype=torch.bool)
+    keep[out] = False
+    assert int(y2[out.cuda()].abs().max()) == 0 and torch.equal(y2[keep.cuda()], y[keep.cuda()])
+
+
+@pytest.mark.parametrize("dt", HALF)
+@pytest.mark.parametrize("T,k,E,N,D", [(1, 8, 12, 2048, 2048), (1, 2, 4, 256, 1024), (1, 2, 4, 130, 2184),
+                                       (3, 2, 8, 72, 4104), (2, 2, 4, 65, 1337), (2, 2, 4, 40, 2565)])
+def test_products_of_few_rows_with_the_depth_shared(T, k, E, N, D, dt):
+    """Four warps share the depth (from 1024 on, or rows of any alignment), one to three rounds each."""
+    _products(T, k, E, N, D, dt)
+
+
+@pytest.mark.parametrize("dt", HALF)
+@pytest.mark.parametrize("T,k,E,N,D", [(3, 2, 8, 100, 520), (3, 2, 8, 100, 776), (5, 3, 8, 33, 1000), (1, 8, 8, 1000, 1544)])
+def test_products_of_few_rows_in_three_rounds_of_depth(T, k, E, N, D, dt):
+    """One warp over the whole depth, past its two rounds in flight."""
+    _products(T, k, E, N, D, dt)
+
+
+@pytest.mark.parametrize("dt", HALF)
+@pytest.mark.parametrize("D", [776, 1032, 1337])
+def test_products_of_few_rows_all_on_one_expert(D, dt):
+    """More rows on one expert than a pass takes (16), beside experts with none."""
+    ids = torch.full((37, 1), 11, dtype=torch.int32)
+    ids[5], ids[30] = 2, -1
+    _products(37, 1, 12, 90, D, dt, ids)
+
+
+@pytest.mark.parametrize("T,k,E,N,D", [(2000, 2, 200, 40, 24), (4300, 2, 500, 24, 40), (10300, 2, 500, 136, 72),
+                                       (900, 2, 4096, 8, 16), (3000, 1, 390, 130, 33)])
+def test_products_of_many_experts(T, k, E, N, D):
+    """More experts than threads in the products' scan of tiles, and more than dW sorts by their rows."""
+    _products(T, k, E, N, D, torch.float16, grads=True)
+
+
+def _route_reference(l, k, score, bias, renorm, dw):
+    """ids, float64 weights and gradients of whole rows (every logit finite)."""
+    key = l.float() if score == "softmax" else 1.0 / (1.0 + torch.exp(-l.float()))
+    key = key if bias is None else key + bias
+    ids = torch.sort(key, dim=1, descending=True, stable=True).indices[:, :k]
+    l, dw = l.double(), dw.double()
+    up = torch.zeros_like(l).scatter_(1, ids, dw)
+    if score == "softmax":
+        over = torch.full_like(l, -INF).scatter(1, ids, l.gather(1, ids)) if renorm else l
+        p = torch.softmax(over, 1)
+        return ids, p.gather(1, ids), p * (up - (up * p).sum(1, keepdim=True)), p * (up.abs() + (up * p).abs().sum(1, keepdim=True))
+    s = torch.sigmoid(l)
+    got = torch.zeros_like(l).scatter_(1, ids, 1.0)
+    slope = s * torch.sigmoid(-l) * got
+    if not renorm:
+        return ids, s.gather(1, ids), up * slope, (up * slope).abs()
+    total = (s * got).sum(1, keepdim=True)
+    mean = (up * s).sum(1, keepdim=True) / total
+    return (ids, (s / total).gather(1, ids), (up - mean) / total * slope,
+            (up.abs() + (up * s).abs().sum(1, keepdim=True) / total) / total * slope)
+
+
+def _check_route(l, k, score, bias, renorm):
+    from mlx_kmeans_b200 import route, route_grad
+    T, E = l.shape
+    dw = torch.randn(T, k, generator=rng(7)).cuda()
+    ids, w = route(l, k, score=score, bias=bias, renormalize=renorm)
+    dl = route_grad(dw, l, ids, score=score, renormalize=renorm)
+    rid, rw, rdl, mag = _route_reference(l, k, score, bias, renorm, dw)
+    assert torch.equal(ids.long(), rid)
+    spread = float(l.float().max() - l.float().min())
+    eps = (spread + 16 + E ** 0.5) * 2.0 ** -23               # as eps_of in test_experts_gpu.py
+    assert torch.all((w.double() - rw).abs() <= eps * rw + 1e-37)
+    tol = U[l.dtype] * rdl.abs() + 4 * (eps + k * 2.0 ** -23) * mag + TINY[l.dtype]
+    assert torch.all((dl.double() - rdl).abs() <= tol)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renorm", [False, True])
+@pytest.mark.parametrize("T,E,k,biased", [(16384, 129, 16, False), (16385, 200, 8, True), (16391, 256, 3, False), (16384, 250, 9, True)])
+def test_route_of_many_rows_of_many_experts(T, E, k, biased, renorm, score, dt):
+    """129 to 256 experts and 16384 rows on: sixteen lanes a row with sixteen experts each."""
+    g = rng(T + E)
+    l = (torch.randn(T, E, generator=g) * 2).to(dt).cuda()
+    _check_route(l, k, score, (torch.randn(E, generator=g) * 0.3).cuda() if biased else None, renorm)
+
+
+@pytest.mark.parametrize("T,E,k", [(70, 8, 2), (70, 32, 8), (70, 64, 4), (70, 64, 8), (70, 128, 8), (70, 128, 16), (70, 33, 20),
+                                   (16390, 200, 8), (70, 256, 20), (70, 500, 9), (70, 1000, 32)])
+@pytest.mark.parametrize("dt", TYPES)
+def test_route_keys_that_differ_in_their_last_bits(T, E, k, dt):
+    """Keys whose upper bits agree (the choice's fast path cuts the lower ones off for the index): float32 logits or
+    biased 16-bit ones next to each other, in some of the rows."""
+    g = rng(E + k)
+    step = torch.stack([torch.randperm(E, generator=g) for _ in range(70)]).repeat((T + 69) // 70, 1)[:T].float()
+    close = (torch.rand(T, 1, generator=g) < 0.5).float()
+    if dt == torch.float32:
+        l = (1.0 + step * 2.0 ** -23) * close + torch.randn(T, E, generator=g) * (1 - close)
+        _check_route(l.cuda(), k, "softmax", None, True)
+        _check_route((-l).cuda(), k, "softmax", None, True)
+    else:
+        l = torch.where(close > 0, torch.ones(T, E), torch.randn(T, E, generator=g)).to(dt)
+        bias = step[0] * 2.0 ** -23 + 0.5
+        _check_route(l.cuda(), k, "softmax", bias.cuda(), True)
+        _check_route((-l).cuda(), k, "softmax", (-bias).cuda(), True)
