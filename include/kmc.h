@@ -361,7 +361,8 @@ int kmc_route_grad(const float *dweights, const void *logits, int dtype, int64_t
 /* Stable grouping of pairs by expert.  ids: rows x choices int32 (labels of a Lloyd pass too: choices = 1); ids outside
  * [0, experts) are left out.  offsets (experts + 1): expert e has positions offsets[e] .. offsets[e + 1] - 1, in
  * increasing (row, choice).  group_row (rows * choices): the row of each position, -1 past offsets[experts].  slot
- * (rows x choices): the position of each pair, or -1.  workspace: kmc_group_bytes(pairs, experts) bytes (may be 0). */
+ * (rows x choices): the position of each pair, or -1.  workspace: kmc_group_bytes(pairs, experts) bytes, 4-byte aligned
+ * (may be 0). */
 size_t kmc_group_bytes(int64_t pairs, int experts);
 int kmc_group_rows(const int32_t *ids, int64_t rows, int choices, int experts, int32_t *offsets, int32_t *group_row,
                    int32_t *slot, void *workspace, size_t ws_bytes, void *stream);

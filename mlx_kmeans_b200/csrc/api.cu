@@ -780,6 +780,16 @@ static int check_dtype(const char* who, int dtype, bool f32) {
     return fail(KMC_ERR_INVALID, "%s: dtype %d is not %s", who, dtype, f32 ? "float32, bfloat16 or float16" : "bfloat16 or float16");
 }
 
+// `need` bytes of workspace that start on a multiple of `align`
+static int check_ws(const char* who, const void* ws, size_t ws_bytes, size_t need, size_t align) {
+    if (need == 0) return KMC_OK;
+    if (!ws || ws_bytes < need)
+        return fail(KMC_ERR_INVALID, "%s: workspace of %zu bytes, need %zu", who, ws ? ws_bytes : (size_t)0, need);
+    if (reinterpret_cast<uintptr_t>(ws) % align != 0)
+        return fail(KMC_ERR_INVALID, "%s: the workspace is not %zu-byte aligned", who, align);
+    return KMC_OK;
+}
+
 // rows of `choices` pairs, counted in int32
 static int check_pairs(const char* who, int64_t rows, int choices) {
     if (rows < 0) return fail(KMC_ERR_INVALID, "%s: rows must be >= 0, got %lld", who, (long long)rows);
@@ -874,8 +884,7 @@ int kmc_group_rows(const int32_t* ids, int64_t rows, int choices, int experts, i
     if (int s = check_experts("kmc_group_rows", experts)) return s;
     if (!offsets || (rows > 0 && (!ids || !group_row || !slot))) return fail(KMC_ERR_INVALID, "kmc_group_rows: null pointer");
     const size_t need = group_bytes(rows * choices, experts);
-    if (need > 0 && (!workspace || ws_bytes < need))
-        return fail(KMC_ERR_INVALID, "kmc_group_rows: workspace of %zu bytes, need %zu", workspace ? ws_bytes : (size_t)0, need);
+    if (int s = check_ws("kmc_group_rows", workspace, ws_bytes, need, 4)) return s;
     cudaError_t e = launch_group(ids, rows * choices, choices, experts, offsets, group_row, slot, workspace,
                                  static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return cuda_fail(e, "kmc_group_rows");
@@ -909,8 +918,7 @@ static int check_expert(const char* who, int64_t pairs, int experts, int n, int 
 
 static int run_expert(const char* who, const ExpertCall& c, size_t ws_bytes, void* stream) {
     const size_t need = expert_bytes(c);
-    if (need > 0 && (!c.ws || ws_bytes < need))
-        return fail(KMC_ERR_INVALID, "%s: workspace of %zu bytes, need %zu", who, c.ws ? ws_bytes : (size_t)0, need);
+    if (int s = check_ws(who, c.ws, ws_bytes, need, 256)) return s;
     cudaError_t e = launch_expert(c, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return cuda_fail(e, who);
     return KMC_OK;
@@ -999,8 +1007,7 @@ int kmc_expert_matmul_dx_rows(const void* dy, const void* w, const int32_t* offs
     if (!w || (rows > 0 && (!dy || !slot || !dx))) return fail(KMC_ERR_INVALID, "%s: null pointer", who);
     if (rows == 0) return KMC_OK;
     const size_t need = kmc_expert_dx_rows_bytes(w, dy, rows, choices, experts, n, d);
-    if (!workspace || ws_bytes < need)
-        return fail(KMC_ERR_INVALID, "%s: workspace of %zu bytes, need %zu", who, workspace ? ws_bytes : (size_t)0, need);
+    if (int s = check_ws(who, workspace, ws_bytes, need, 256)) return s;
     const size_t front = dx_positions_bytes(rows * choices, choices, d);
     ExpertCall c = dx_call(dy, w, rows * choices, experts, n, d);
     c.dtype = dtype;
@@ -1133,9 +1140,7 @@ int kmc_combine_grad_slots(const void* dout, const void* y, int dtype, int64_t r
         return fail(KMC_ERR_INVALID, "kmc_combine_grad_slots: null pointer");
     if (rows == 0) return KMC_OK;
     const size_t need = kmc_combine_bytes(rows, choices);
-    if (!workspace || ws_bytes < need)
-        return fail(KMC_ERR_INVALID, "kmc_combine_grad_slots: workspace of %zu bytes, need %zu",
-                    workspace ? ws_bytes : (size_t)0, need);
+    if (int s = check_ws("kmc_combine_grad_slots", workspace, ws_bytes, need, 4)) return s;
     return run_combine_grad("kmc_combine_grad_slots", dout, y, dtype, rows, choices, width, slot, weights, nullptr,
                             static_cast<int32_t*>(workspace), dy, dweights, stream);
 }

@@ -58,3 +58,18 @@ def test_arguments_of_other_types():
     for f in calls:
         with pytest.raises(ValueError, match="CUDA tensor|RowGroups"):
             f()
+
+
+def test_workspaces_off_their_alignment():
+    """A workspace that does not start where the header says is refused: its vectors would be read off their boundary."""
+    _l, L = lib()
+    bad, big = _l.KMC_ERR_INVALID, 1 << 20
+    x = P + 2                                                  # rows off 16 bytes: copied to the workspace
+    for at in (P + 4, P + 16, P + 128):
+        for rc in (L.kmc_expert_matmul(x, 400, 16, None, P, P, 400, 4, 8, 16, 1, P, at, big, P, None),
+                   L.kmc_expert_matmul_dx(x, P, P, 400, 4, 8, 16, 1, P, at, big, P, None),
+                   L.kmc_expert_matmul_dw(x, P, 400, 16, None, P, 400, 4, 8, 16, 1, P, at, big, P, None),
+                   L.kmc_expert_matmul_dx_rows(P, P, P, P, 4, 2, 4, 8, 16, 1, P, at, big, P, None)):
+            assert rc == bad and b"256" in L.kmc_last_error()
+    assert L.kmc_group_rows(P, 1 << 19, 2, 256, P, P, P, P + 2, big, None) == bad and b"4-byte" in L.kmc_last_error()
+    assert L.kmc_combine_grad_slots(P, P, 0, 4, 2, 8, P, None, P, P, P + 2, 32, None) == bad and b"4-byte" in L.kmc_last_error()
