@@ -45,7 +45,8 @@ class RowGroups(NamedTuple):
     offsets (n_experts + 1): expert e has the positions offsets[e] .. offsets[e + 1] - 1.
     rows (pairs): the row each position reads, -1 past offsets[-1].
     slot (rows, choices) or (rows,): the position of each pair, -1 for a pair that was left out.  A caller may set
-    further ones to -1 (experts over their capacity): combine_rows and the gradients then leave those pairs out.
+    further ones to -1 before the first use (experts over their capacity): combine_rows leaves those pairs out, and its
+    gradient at their positions is 0, so nothing of them reaches the gradients of expert_matmul.
     """
     offsets: torch.Tensor
     rows: torch.Tensor
@@ -200,8 +201,8 @@ def expert_matmul(x, w, groups, *, gather=True):
 
 
 def expert_matmul_grad(dy, x, w, groups, *, gather=True):
-    """The gradients of expert_matmul for dy (positions, n): dx in x's shape (with gather=True a row's positions are
-    summed in float32 and the sum is rounded) and dw in w's; an expert with no position gets a dw of zeros."""
+    """The gradients of expert_matmul for dy (positions, n): dx in x's shape (with gather=True the positions of a row's
+    slots are summed in float32 and the sum is rounded) and dw in w's; an expert with no position gets a dw of zeros."""
     _tensors((dy, "dy"), (x, "x"), (w, "w"))
     if x.ndim == 2 and w.ndim == 3 and x.shape[1] != w.shape[2]:
         raise ValueError(f"x has {x.shape[1]} columns, the matrices {w.shape[2]}")

@@ -536,3 +536,21 @@ def test_route_keys_that_differ_in_their_last_bits(T, E, k, dt):
         bias = step[0] * 2.0 ** -23 + 0.5
         _check_route(l.cuda(), k, "softmax", bias.cuda(), True)
         _check_route((-l).cuda(), k, "softmax", (-bias).cuda(), True)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("T,k,H", [(3, 2, 33), (130, 8, 512)])
+def test_combine_grad_of_whole_plans_through_the_c_entry(T, k, H, dt):
+    """kmc_combine_grad, told where the pairs end, gives what kmc_combine_grad_slots finds out."""
+    from mlx_kmeans_b200 import _lib, combine_rows_grad
+    L, g = _lib.load(), rng(T)
+    groups = plan(T, k, max(4, k), T, drop=0.2)
+    y, dout = torch.randn(T * k, H, generator=g).to(dt).cuda(), torch.randn(T, H, generator=g).to(dt).cuda()
+    w = torch.rand(T, k, generator=g).cuda()
+    want_dy, want_dw = combine_rows_grad(dout, y, groups, w)
+    dy, dw = torch.full_like(y, float("nan")), torch.full_like(w, float("nan"))
+    kind = {torch.float32: _lib.KMC_F32, torch.bfloat16: _lib.KMC_BF16, torch.float16: _lib.KMC_F16}[dt]
+    _lib.check(L.kmc_combine_grad(dout.data_ptr(), y.data_ptr(), kind, T, k, H, groups.slot.data_ptr(), w.data_ptr(),
+                                  groups.offsets[-1:].data_ptr(), dy.data_ptr(), dw.data_ptr(),
+                                  torch.cuda.current_stream().cuda_stream), "kmc_combine_grad")
+    assert torch.equal(dy, want_dy) and torch.equal(dw, want_dw)
