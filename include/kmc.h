@@ -376,7 +376,8 @@ int kmc_group_rows(const int32_t *ids, int64_t rows, int choices, int experts, i
  * rows * choices; a slot of -1 adds nothing) summed in float32 and rounded once.  Its workspace is
  * kmc_expert_dx_rows_bytes, 256-byte aligned: the positions' gradients, float32 with more than one choice a row, and
  * what kmc_expert_bytes gives for kmc_expert_matmul_dx.
- * kmc_expert_matmul_dw: dW (experts x n x d) = sum over an expert's positions of dy x^T; 0 for an expert with none.
+ * kmc_expert_matmul_dw: dW (experts x n x d) = sum over an expert's positions of dy x^T; 0 for an expert with none.  (One
+ * float32 sum: past 2^24 positions of an expert give them in parts.)
  * workspace: kmc_expert_bytes bytes for the call's operands (NULL for one it does not take), 256-byte aligned: room for
  * x in grouped order where that is read faster, and for padded copies of operands that do not start on 16 bytes or have
  * rows that are not a multiple of 8 elements apart; may be 0.  error (an int32 that the device can

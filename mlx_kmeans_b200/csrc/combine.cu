@@ -10,7 +10,7 @@
 // Memory bound.  Forward: one thread per 16 bytes of out, its k reads of y independent and in flight together; each
 // row of y is read once and each row of out written once.  Backward: one warp per pair reads dout_t (the k warps of a
 // row run side by side, so it comes from L1 / L2 after the first) and y's row once and writes dy's row.  16384 rows of 8
-// choices, 2048 features, bfloat16: both in 277 us, where their bytes (1.74 GB) take 266 at the copy bandwidth.
+// choices, 2048 features, bfloat16: both in 281 us, where their bytes (1.74 GB) take 266 at the copy bandwidth.
 #include <type_traits>
 
 #include "common.cuh"

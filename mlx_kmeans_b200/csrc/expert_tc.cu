@@ -19,9 +19,12 @@
 // positions past a group's end in dW are loaded that way, so no other group's value (a NaN, say) enters the sum; in
 // forward and dx a neighbour's row can only reach columns that are not stored.
 //
-// Measured (bfloat16): 8192^3 in one group 805 us, 1366 TFLOP/s; 65536 rows of 64 groups, 2048 x 2048, forward and dx 1110
-// TFLOP/s, dW 1050; without its loads the first takes 682 us and without L2 misses 755 us, so operands on their way to
-// shared memory bound it (32 KB a stage and CTA, about 45 bytes a cycle), then the tensor cores.
+// Measured (bfloat16, the kernel alone in short bursts): 8192^3 in one group 805 us, 1366 TFLOP/s; 65536 rows of 64
+// groups, 2048 x 2048, forward and dx 1110 TFLOP/s, dW 1050 (a forward pass in a row of passes, the copy of x in grouped
+// order included and under the power limit: 666 us, 825); 16396 rows of 16 groups, 1536 x 2048, 1000 TFLOP/s, dx with
+// float32 results 930, the tensor pipe 53 to 58% busy.  Without its loads the first takes 682 us and without L2 misses
+// 755 us, so operands on their way to shared memory bound it (32 KB a stage and CTA, about 45 bytes a cycle), then the
+// tensor cores.
 //
 // Kernel layout (persistent, one CTA per SM): warp 0 loads (TMA), warp 1 issues the MMAs (64 deep a stage; in a pair
 // the leader's alone), warps 2-5 store the finished accumulator while the next one is computed (two accumulators in

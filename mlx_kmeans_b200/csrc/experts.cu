@@ -9,7 +9,7 @@
 // 256 positions spent four times as long on them as on its MMAs (8192 x 8 of 64 experts, 2048 x 2048: 2365 us, from
 // grouped rows 529 us), and warps that gather with 16-byte asynchronous copies took 1190 us (the hand-over of a stage
 // from copies to tensor cores takes longer than its MMAs).  With more rows an expert, and for dW, x is copied in grouped
-// order first: 70 us there, what writing it takes, of 560 in all (32 experts, 2048 x 2048: 6 rows each 57.4 us gathered,
+// order first: 70 us there, what writing it takes, of 565 in all (32 experts, 2048 x 2048: 6 rows each 57.4 us gathered,
 // 60.4 copied; 32 rows each 84.1 and 61.1).
 #include "common.cuh"
 #include "experts.cuh"
@@ -28,7 +28,10 @@ size_t a256(size_t v) { return (v + 255) & ~size_t(255); }
 // Forward products of few rows take expert_rows.cu: up to four rows an expert at any size, up to sixteen where all the
 // matrices together are small and the tensor-core kernel's set-up counts (device time, 16-bit, rows against tiles:
 // 2048 x 2048, 8 of 64 experts: 1 row each 16 us against 19, 4 each 94 against 95, 16 each 225 against 111;
-// 512 x 512, 8 experts: 1 to 4 rows each 3 us against 8, 16 each 5 against 9, 32 each 10 against 10).
+// 512 x 512, 8 experts: 1 to 4 rows each 3 us against 8, 16 each 5 against 9, 32 each 10 against 10).  The rule does not
+// look at alignment or at the number of features, and misses the faster side there: rows read element by element, 333 x 515,
+// 192 pairs of 32 experts 18.5 against 15.5 and 256 of 64 27.0 against 24.6 (48 of 32 11.5 against 15.4, 128 of 8 11.1
+// against 11.5); few features, 64 x 1024, 256 pairs of 8, which go to the tiles, 5.5 against 13.1.
 bool by_rows(const ExpertCall& c) {
     if (c.kind != kExpertForward) return false;
     const int64_t used = c.pairs < c.experts ? c.pairs : c.experts;
