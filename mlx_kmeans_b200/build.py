@@ -3,7 +3,8 @@ tensors to the routed-experts entry points, csrc/bind_experts.cpp).
 
     python -m mlx_kmeans_b200.build          # or: python mlx_kmeans_b200/build.py
 
-nvcc cross-compiles without a GPU, so this runs on any machine with the CUDA 12.9 toolkit.  Objects are
+nvcc cross-compiles without a GPU, so this runs on any machine with the CUDA 12.9 toolkit (without torch, libkmc.so
+alone is built).  Objects are
 compiled in parallel and relinked only when a source or header is newer than the library.
 """
 import concurrent.futures
@@ -84,12 +85,17 @@ def build(verbose=False, force=False, extra=()):
 
 
 def build_binding(verbose=False, force=False):
-    """Compile csrc/bind_experts.cpp against the installed torch and link it to libkmc.so. Returns its path."""
+    """Compile csrc/bind_experts.cpp against the installed torch and link it to libkmc.so. Returns its path, or None on a
+    machine without torch, where libkmc.so alone is of use."""
     deps = [BIND_SRC, os.path.join(ROOT, "include", "kmc.h")]
     if not force and os.path.exists(BIND) and all(os.path.getmtime(p) <= os.path.getmtime(BIND) for p in deps):
         return BIND
-    import torch
-    base = os.path.join(os.path.dirname(torch.__file__))
+    try:
+        import torch
+    except ImportError:
+        print("torch is not installed: the module _experts is not built", file=sys.stderr)
+        return None
+    base = os.path.dirname(torch.__file__)
     inc = [os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"),
            os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include"), sysconfig.get_paths()["include"]]
     tmp = BIND + ".tmp"
